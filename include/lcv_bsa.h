@@ -455,6 +455,103 @@ int lcv_bsa_prepare_qkv(const void* q_in, const void* k_in, const void* v_in,
                         lcv_bsa_strides k_norm_strides, float* qbar,
                         float* kbar, void* stream);
 
+/*
+ * Rotary positions with several axes at positions given per token (rope_3d.py:
+ * 37-128 rotates the tokens of one whole grid): with theta = position[s][a] *
+ * base^(-2 i / dims[a]) for pair i of axis a,
+ *   out[2p] = x[2p] cos theta - x[2p+1] sin theta,
+ *   out[2p+1] = x[2p] sin theta + x[2p+1] cos theta,
+ * and with -theta where `inverse` is set: the gradient.  x, out [B,H,S,D], D % 8
+ * == 0, D <= 256, rows on 16-byte boundaries; out may be x itself.  positions
+ * [B or 1, S, axes] of type int32 (0), int64 (1) or fp32 (2), the axes next to one
+ * another, strides in elements (batch stride 0: shared).  dims (host memory) holds
+ * the axes' dims: even, summing to D.  Angles are taken in 64 bits.
+ */
+int lcv_bsa_rope_nd(const void* x, int dtype, int64_t B, int64_t H, int64_t S,
+                    int64_t D, lcv_bsa_strides xs, const void* positions,
+                    int position_type, int64_t pos_stride_b,
+                    int64_t pos_stride_s, const int64_t* dims, int64_t axes,
+                    double base, int inverse, void* out, lcv_bsa_strides os,
+                    void* stream);
+
+/*
+ * A KV cache in 8 bits: keys k8 [B,H,capacity,D], values v8 [B,H,capacity/64,D,64]
+ * (each block of 64 tokens transposed: the order in which P V reads them), e4m3
+ * bytes, and one scale for the keys and one for the values of each block
+ * [B,H,capacity/64], powers of two in [2^-60, 2^60].  Dense; k8 and v8 16-byte
+ * aligned; D in {64, 128}; capacity a multiple of 64.
+ */
+typedef struct lcv_bsa_cache8 {
+  void* k8;
+  void* v8;
+  float* k_scale;
+  float* v_scale;
+  int64_t B, H, capacity, D;
+} lcv_bsa_cache8;
+
+/*
+ * Writes rows k, v [B,H,S,D] (fp16, bf16, fp32) into the cache: item b's first
+ * counts[b] rows (all S if counts is null) become its tokens start[b] .. .  A
+ * block's scale becomes the least power of two that brings the largest finite of
+ * its new rows within 448, and no less than it was where the block keeps rows
+ * before start[b]; those are rounded again if it grows.  Rounding is to nearest,
+ * ties to even; infinities, NaN and what lies beyond the scales' range become NaN.
+ * Rows past the capacity, and items with a negative start, are left out; bytes
+ * behind the last new row stay as they were.  start and counts are read on the
+ * device.
+ */
+int lcv_bsa_cache_append(lcv_bsa_cache8 c, const void* k, const void* v,
+                         int dtype, int64_t S, lcv_bsa_strides ks,
+                         lcv_bsa_strides vs, const int32_t* start,
+                         const int32_t* counts, void* stream);
+
+/*
+ * Attention of q [B,Hq,S,D] (fp16 / bf16, Hq a multiple of the cache's H: query
+ * head h reads key head h / (Hq / H)) over the first lengths[b] tokens of item b's
+ * cache.  q_lens[b] (null: S) of its queries are real, and with `causal` set query
+ * i sees the tokens up to lengths[b] - q_lens[b] + i: the real queries are the last
+ * tokens.  out [B,Hq,S,D] and, if given, lse [B,Hq,S] (natural log of the sum of
+ * exp(sm_scale q.k)); rows that see no token get zeros and -inf.  max_len bounds
+ * the lengths (longer ones count as max_len).  sm_scale >= 0; rows on 16-byte
+ * boundaries.  lengths and q_lens are read on the device.  The workspace holds the
+ * parts of a split walk.
+ */
+size_t lcv_bsa_cached_attn_workspace_bytes(int64_t Hq, int64_t S,
+                                           lcv_bsa_cache8 c, int64_t max_len);
+int lcv_bsa_cached_attn(const void* q, int dtype, int64_t Hq, int64_t S,
+                        lcv_bsa_strides qs, lcv_bsa_cache8 c,
+                        const int32_t* lengths, const int32_t* q_lens,
+                        int causal, float sm_scale, int64_t max_len, void* out,
+                        lcv_bsa_strides os, float* lse, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
+ * What each cached token got from these queries: out[b,h,j] = weights[b,h,j] +
+ * the sum over the queries of key head h that see token j of exp(sm_scale q.k_j -
+ * lse), with lse from lcv_bsa_cached_attn.  weights (null: zeros) and out are
+ * [B,H,capacity] fp32, and may be one.  The sums' order is fixed.
+ */
+int lcv_bsa_attention_weights(const void* q, int dtype, int64_t Hq, int64_t S,
+                              lcv_bsa_strides qs, lcv_bsa_cache8 c,
+                              const int32_t* lengths, const int32_t* q_lens,
+                              int causal, float sm_scale, int64_t max_len,
+                              const float* lse, const float* weights,
+                              float* out, void* stream);
+
+/*
+ * Cuts a cache down: of each head's lengths[b] tokens the newest `recent` stay and
+ * of the others those of the largest weights [B,H,capacity] (equal ones: the lowest
+ * token first; NaN below everything), keep in all, in their order, into dst (another
+ * cache of the same B, H, D; capacity >= keep), whose blocks get the least scales for
+ * their rows; rows behind the last are zero, and a block without rows has scale 1.
+ * kept [B,H,keep] lists the tokens (-1 behind the last), new_weights
+ * [B,H,dst.capacity] their weights (0 behind), new_lengths [B] = min(length, keep).
+ */
+int lcv_bsa_cache_evict(lcv_bsa_cache8 src, const int32_t* lengths,
+                        const float* weights, int64_t keep, int64_t recent,
+                        lcv_bsa_cache8 dst, float* new_weights, int32_t* kept,
+                        int32_t* new_lengths, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,7 @@
 #include <mutex>
 
 #include "bsa_common.h"
+#include "cache_common.h"
 
 #define LCV_BSA_VERSION "lcv_bsa 0.1.0 gfx950"
 
@@ -984,6 +985,200 @@ int lcv_bsa_prepare_qkv(const void* q_in, const void* k_in, const void* v_in, in
                                                rope_table, (int)rope_table_len, eps,
                                                (hipStream_t)stream),
                        "lcv_bsa_prepare_qkv");
+}
+
+}  // extern "C"
+
+namespace {
+
+// A cache's shape, pointers and limits: every (item, head, block) numbered in 31 bits, twice over.
+int check_cache(const char* name, const lcv_bsa_cache8& c) {
+  if (!c.k8 || !c.v8 || !c.k_scale || !c.v_scale) return fail(LCV_BSA_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (c.B <= 0 || c.H <= 0 || c.capacity <= 0)
+    return fail(LCV_BSA_ERR_INVALID_ARG, "%s: B, H, capacity must be positive (got %lld, %lld, %lld)", name,
+                (long long)c.B, (long long)c.H, (long long)c.capacity);
+  if (c.D != 64 && c.D != 128)
+    return fail(LCV_BSA_ERR_UNSUPPORTED, "%s: the 8-bit cache holds head dims 64 and 128 (got %lld)", name,
+                (long long)c.D);
+  if (c.capacity % lcv::kCacheBlock)
+    return fail(LCV_BSA_ERR_SHAPE, "%s: capacity %lld is not a multiple of %d", name, (long long)c.capacity,
+                lcv::kCacheBlock);
+  if (c.capacity > ((int64_t)1 << 30) || c.B > kI32Max || c.H > kI32Max || c.B * c.H > kI32Max ||
+      c.B * c.H * (c.capacity / lcv::kCacheBlock) > kI32Max / 2)
+    return fail(LCV_BSA_ERR_UNSUPPORTED, "%s: too many blocks", name);
+  if (((uintptr_t)c.k8 | (uintptr_t)c.v8) & 15u)
+    return fail(LCV_BSA_ERR_LAYOUT, "%s: k8 and v8 must be 16-byte aligned", name);
+  return LCV_BSA_OK;
+}
+
+lcv::Cache8 cache8(const lcv_bsa_cache8& c) {
+  return {(uint8_t*)c.k8, (uint8_t*)c.v8, c.k_scale, c.v_scale, (int32_t)c.B, (int32_t)c.H,
+          (int32_t)(c.capacity / lcv::kCacheBlock)};
+}
+
+// What the attention over a cache and its weights have in common; fills a.
+int check_cache_attn(const void* q, int dtype, int64_t Hq, int64_t S, const lcv_bsa_strides& qs,
+                     const lcv_bsa_cache8& c, const int32_t* lengths, const int32_t* q_lens, int causal,
+                     float sm_scale, int64_t max_len, lcv::CacheAttn* a) {
+  int st = check_cache("cache", c);
+  if (st) return st;
+  if (!q || !lengths) return fail(LCV_BSA_ERR_INVALID_ARG, "null pointer");
+  if (dtype != LCV_BSA_F16 && dtype != LCV_BSA_BF16)
+    return fail(LCV_BSA_ERR_DTYPE, "attention over the 8-bit cache takes fp16 and bf16 queries");
+  if (Hq <= 0 || S <= 0) return fail(LCV_BSA_ERR_INVALID_ARG, "query heads and rows must be positive");
+  if (Hq % c.H || Hq / c.H > kI32Max || S > kI32Max)
+    return fail(LCV_BSA_ERR_SHAPE, "%lld query heads are not a multiple of the cache's %lld", (long long)Hq,
+                (long long)c.H);
+  if (max_len <= 0 || max_len > c.capacity)
+    return fail(LCV_BSA_ERR_INVALID_ARG, "max_len=%lld must be in [1, capacity=%lld]", (long long)max_len,
+                (long long)c.capacity);
+  if (!(sm_scale >= 0.0f) || !std::isfinite(sm_scale))
+    return fail(LCV_BSA_ERR_UNSUPPORTED, "sm_scale must be finite and >= 0");
+  if ((Hq / c.H) * S > kI32Max / 64 || c.B * c.H * (((Hq / c.H) * S + 15) / 16) > kI32Max / 2)
+    return fail(LCV_BSA_ERR_UNSUPPORTED, "too many query rows");
+  if ((st = check_rows("q", q, qs, c.D))) return st;
+  *a = lcv::CacheAttn{};
+  a->c = cache8(c);
+  a->q = tensor4(q, qs);
+  a->lengths = lengths;
+  a->q_lens = q_lens;
+  a->group = (int32_t)(Hq / c.H);
+  a->S = (int32_t)S;
+  a->max_len = (int32_t)max_len;
+  a->causal = causal ? 1 : 0;
+  a->scale_log2 = (float)((double)sm_scale * 1.4426950408889634);
+  return LCV_BSA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lcv_bsa_rope_nd(const void* x, int dtype, int64_t B, int64_t H, int64_t S, int64_t D, lcv_bsa_strides xs,
+                    const void* positions, int position_type, int64_t pos_stride_b, int64_t pos_stride_s,
+                    const int64_t* dims, int64_t axes, double base, int inverse, void* out, lcv_bsa_strides os,
+                    void* stream) {
+  if (!x || !positions || !dims || !out) return fail(LCV_BSA_ERR_INVALID_ARG, "null pointer");
+  if (!dtype_ok(dtype)) return fail(LCV_BSA_ERR_DTYPE, "unknown dtype %d", dtype);
+  if (position_type < lcv::kPosI32 || position_type > lcv::kPosF32)
+    return fail(LCV_BSA_ERR_DTYPE, "unknown position type %d", position_type);
+  if (B <= 0 || H <= 0 || S <= 0 || axes <= 0)
+    return fail(LCV_BSA_ERR_INVALID_ARG, "B, H, S and the number of axes must be positive");
+  if (D <= 0 || D % 8 || D > 2 * lcv::kRopeMaxPairs)
+    return fail(LCV_BSA_ERR_UNSUPPORTED, "rope_nd supports head dims that are multiples of 8 up to %d (got %lld)",
+                2 * lcv::kRopeMaxPairs, (long long)D);
+  if (axes > D / 2 || !(base > 0.0) || !std::isfinite(base))
+    return fail(LCV_BSA_ERR_INVALID_ARG, "at most D / 2 axes and a positive base");
+  if (pos_stride_b < 0 || pos_stride_s < 0) return fail(LCV_BSA_ERR_LAYOUT, "position strides must be non-negative");
+  if (B > kI32Max || H > kI32Max || S > kI32Max || B * H > kI32Max || B * S > ((int64_t)1 << 33) || B * H * S > ((int64_t)1 << 40))
+    return fail(LCV_BSA_ERR_UNSUPPORTED, "tensor too large");
+  int st;
+  if ((st = check_strides("x", xs, D)) || (st = check_strides("out", os, D))) return st;
+  const int vec = 16 / elem_bytes(dtype);
+  if (!vec_aligned(x, xs, vec) || !vec_aligned(out, os, vec))
+    return fail(LCV_BSA_ERR_LAYOUT, "x and out rows must start on 16-byte boundaries");
+  lcv::RopeNd r{};
+  int64_t pair = 0;
+  for (int64_t a = 0; a < axes; ++a) {
+    if (dims[a] <= 0 || dims[a] % 2 || pair + dims[a] / 2 > D / 2)
+      return fail(LCV_BSA_ERR_SHAPE, "the axes' dims must be even, positive and sum to D=%lld", (long long)D);
+    for (int64_t i = 0; i < dims[a] / 2; ++i, ++pair) {
+      r.axis[pair] = (uint8_t)a;
+      r.turns[pair] = std::pow(base, -2.0 * (double)i / (double)dims[a]) / 6.283185307179586;
+    }
+  }
+  if (pair != D / 2)
+    return fail(LCV_BSA_ERR_SHAPE, "the axes' dims must be even, positive and sum to D=%lld", (long long)D);
+  r.x = tensor4(x, xs);
+  r.y = tensor4(out, os);
+  r.positions = positions;
+  r.pos_sb = pos_stride_b;
+  r.pos_ss = pos_stride_s;
+  r.B = (int32_t)B;
+  r.H = (int32_t)H;
+  r.S = (int32_t)S;
+  r.pairs = (int32_t)(D / 2);
+  r.sign = inverse ? -1.0f : 1.0f;
+  return launch_status(lcv::launch_rope_nd(r, dtype, position_type, (hipStream_t)stream), "lcv_bsa_rope_nd");
+}
+
+int lcv_bsa_cache_append(lcv_bsa_cache8 c, const void* k, const void* v, int dtype, int64_t S, lcv_bsa_strides ks,
+                         lcv_bsa_strides vs, const int32_t* start, const int32_t* counts, void* stream) {
+  int st = check_cache("cache", c);
+  if (st) return st;
+  if (!k || !v || !start) return fail(LCV_BSA_ERR_INVALID_ARG, "null pointer");
+  if (!dtype_ok(dtype)) return fail(LCV_BSA_ERR_DTYPE, "unknown dtype %d", dtype);
+  if (S <= 0) return fail(LCV_BSA_ERR_INVALID_ARG, "S must be positive");
+  if (S > c.capacity || c.B * c.H * ((S + 126) / 64) > kI32Max / 2)
+    return fail(LCV_BSA_ERR_SHAPE, "%lld rows for a cache of %lld tokens", (long long)S, (long long)c.capacity);
+  if ((st = check_strides("k", ks, c.D)) || (st = check_strides("v", vs, c.D))) return st;
+  const int vec = 16 / elem_bytes(dtype);
+  if (!vec_aligned(k, ks, vec) || !vec_aligned(v, vs, vec))
+    return fail(LCV_BSA_ERR_LAYOUT, "k and v rows must start on 16-byte boundaries");
+  return launch_status(lcv::launch_cache_append(cache8(c), tensor4(k, ks), tensor4(v, vs), dtype, (int)S, (int)c.D,
+                                                start, counts, (hipStream_t)stream),
+                       "lcv_bsa_cache_append");
+}
+
+size_t lcv_bsa_cached_attn_workspace_bytes(int64_t Hq, int64_t S, lcv_bsa_cache8 c, int64_t max_len) {
+  if (c.B <= 0 || c.H <= 0 || Hq < c.H || S <= 0 || max_len <= 0 || Hq * S > kI32Max) return 0;
+  lcv::CacheAttn a{};
+  a.c.B = (int32_t)c.B;
+  a.c.H = (int32_t)c.H;
+  a.c.nb = (int32_t)(c.capacity / lcv::kCacheBlock);
+  a.group = (int32_t)(Hq / c.H);
+  a.S = (int32_t)S;
+  a.max_len = (int32_t)max_len;
+  return lcv::cache_attn_workspace(a, (int)c.D);
+}
+
+int lcv_bsa_cached_attn(const void* q, int dtype, int64_t Hq, int64_t S, lcv_bsa_strides qs, lcv_bsa_cache8 c,
+                        const int32_t* lengths, const int32_t* q_lens, int causal, float sm_scale, int64_t max_len,
+                        void* out, lcv_bsa_strides os, float* lse, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  lcv::CacheAttn a;
+  int st = check_cache_attn(q, dtype, Hq, S, qs, c, lengths, q_lens, causal, sm_scale, max_len, &a);
+  if (st) return st;
+  if (!out) return fail(LCV_BSA_ERR_INVALID_ARG, "null pointer");
+  if ((st = check_rows("out", out, os, c.D))) return st;
+  a.out = tensor4(out, os);
+  a.lse = lse;
+  const size_t need = lcv::cache_attn_workspace(a, (int)c.D);
+  if (workspace_bytes < need || (need && (!workspace || (uintptr_t)workspace % 16)))
+    return fail(LCV_BSA_ERR_INVALID_ARG, "workspace of %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
+  a.workspace = workspace;
+  return launch_status(lcv::launch_cache_attn(a, dtype, (int)c.D, (hipStream_t)stream), "lcv_bsa_cached_attn");
+}
+
+int lcv_bsa_attention_weights(const void* q, int dtype, int64_t Hq, int64_t S, lcv_bsa_strides qs, lcv_bsa_cache8 c,
+                              const int32_t* lengths, const int32_t* q_lens, int causal, float sm_scale,
+                              int64_t max_len, const float* lse, const float* weights, float* out, void* stream) {
+  lcv::CacheAttn a;
+  const int st = check_cache_attn(q, dtype, Hq, S, qs, c, lengths, q_lens, causal, sm_scale, max_len, &a);
+  if (st) return st;
+  if (!lse || !out) return fail(LCV_BSA_ERR_INVALID_ARG, "null pointer");
+  a.lse = const_cast<float*>(lse);
+  return launch_status(lcv::launch_cache_weights(a, dtype, (int)c.D, weights, out, (hipStream_t)stream),
+                       "lcv_bsa_attention_weights");
+}
+
+int lcv_bsa_cache_evict(lcv_bsa_cache8 src, const int32_t* lengths, const float* weights, int64_t keep, int64_t recent,
+                        lcv_bsa_cache8 dst, float* new_weights, int32_t* kept, int32_t* new_lengths, void* stream) {
+  int st;
+  if ((st = check_cache("cache", src)) || (st = check_cache("out", dst))) return st;
+  if (!lengths || !weights || !new_weights || !kept || !new_lengths)
+    return fail(LCV_BSA_ERR_INVALID_ARG, "null pointer");
+  if (src.B != dst.B || src.H != dst.H || src.D != dst.D)
+    return fail(LCV_BSA_ERR_SHAPE, "the new cache must have the old one's items, heads and head dim");
+  if (keep <= 0 || keep > dst.capacity || recent < 0 || recent > keep)
+    return fail(LCV_BSA_ERR_INVALID_ARG, "keep=%lld must be in [1, %lld] and recent=%lld in [0, keep]",
+                (long long)keep, (long long)dst.capacity, (long long)recent);
+  if (src.k8 == dst.k8 || src.v8 == dst.v8 || src.k_scale == dst.k_scale || src.v_scale == dst.v_scale ||
+      weights == new_weights)
+    return fail(LCV_BSA_ERR_INVALID_ARG, "an eviction does not work in place");
+  return launch_status(lcv::launch_cache_evict(cache8(src), lengths, weights, (int)keep, (int)recent, cache8(dst),
+                                               new_weights, kept, new_lengths, (int)src.D, (hipStream_t)stream),
+                       "lcv_bsa_cache_evict");
 }
 
 }  // extern "C"

@@ -25,6 +25,8 @@ from .block_sparse_attention_hip import (  # noqa: F401
     reshape_to_block_major,
 )
 from .prepare import prepare_qk, prepare_qkv, rope_table  # noqa: F401
+from .rope_positions import grid_positions, rope_nd  # noqa: F401
+from .kv_cache import KVCache8, attention_weights, cache_append, cache_evict, cached_attention  # noqa: F401
 from .attention import BSAAttention, backend_from_env  # noqa: F401
 from .dit import BSAModelMixin, apply_bsa_params, disable_bsa, enable_bsa  # noqa: F401
 

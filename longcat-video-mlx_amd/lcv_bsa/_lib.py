@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "liblcv_bsa.so"
@@ -44,6 +44,12 @@ class Grid(ctypes.Structure):
     """lcv_bsa_grid: latent grid (T, Hl, Wl) of the RoPE positions."""
 
     _fields_ = [(n, c_int64) for n in ("T", "Hl", "Wl")]
+
+
+class Cache8(ctypes.Structure):
+    """lcv_bsa_cache8: an 8-bit KV cache."""
+
+    _fields_ = [(n, c_void_p) for n in ("k8", "v8", "k_scale", "v_scale")] + [(n, c_int64) for n in ("B", "H", "capacity", "D")]
 
 
 _SIGNATURES = {
@@ -105,6 +111,17 @@ _SIGNATURES = {
                                     c_void_p, c_void_p, c_float, Grid, c_void_p, c_int64, Geom, Geom,
                                     c_void_p, c_void_p, c_void_p, c_void_p, Strides, Strides, Strides, Strides,
                                     c_void_p, c_void_p, c_void_p]),
+    "lcv_bsa_rope_nd": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, Strides, c_void_p, c_int, c_int64,
+                                c_int64, c_void_p, c_int64, c_double, c_int, c_void_p, Strides, c_void_p]),
+    "lcv_bsa_cache_append": (c_int, [Cache8, c_void_p, c_void_p, c_int, c_int64, Strides, Strides, c_void_p, c_void_p,
+                                     c_void_p]),
+    "lcv_bsa_cached_attn_workspace_bytes": (c_size_t, [c_int64, c_int64, Cache8, c_int64]),
+    "lcv_bsa_cached_attn": (c_int, [c_void_p, c_int, c_int64, c_int64, Strides, Cache8, c_void_p, c_void_p, c_int,
+                                    c_float, c_int64, c_void_p, Strides, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "lcv_bsa_attention_weights": (c_int, [c_void_p, c_int, c_int64, c_int64, Strides, Cache8, c_void_p, c_void_p, c_int,
+                                          c_float, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "lcv_bsa_cache_evict": (c_int, [Cache8, c_void_p, c_void_p, c_int64, c_int64, Cache8, c_void_p, c_void_p, c_void_p,
+                                    c_void_p]),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -158,6 +175,6 @@ def check(status: int, what: str) -> None:
 
 
 __all__ = [
-    "BF16", "F16", "F32", "Geom", "Grid", "Strides", "EXPORTED", "BSALibraryError", "LIB_PATH",
+    "BF16", "Cache8", "F16", "F32", "Geom", "Grid", "Strides", "EXPORTED", "BSALibraryError", "LIB_PATH",
     "check", "load", "version",
 ]

@@ -1,0 +1,309 @@
+"""A KV cache held in 8 bits, and what writes, reads, weighs and shrinks it.
+
+The reference keeps a continuation's cache in 16 bits (longcat_video/models/
+attention.py:191-201, 235-275), for every layer through every denoising step.
+``KVCache8`` holds e4m3 bytes with one power-of-two scale per block of 64 tokens
+and head: half the memory, and half the bytes of every read.
+
+* ``cache_append`` writes new keys and values (at any token, ragged batches);
+* ``cached_attention`` attends to it: single tokens, prompts, frames of a video,
+  grouped heads, causal or not;
+* ``attention_weights`` adds up what attention each cached token got;
+* ``cache_evict`` cuts the cache down to its heaviest and its newest tokens.
+
+Lengths and positions are int32 tensors that the kernels read on the device, so
+every call can be captured into a graph and replayed as they move on; a plain
+int stands for the same number for every item.  There is no gradient through
+the cache.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Union
+
+import torch
+
+from . import _lib
+from .block_sparse_attention import _dtype_code, _require_device, _stream
+from .rope_positions import on_device, rows_of
+
+__all__ = ["KVCache8", "cache_append", "cached_attention", "attention_weights", "cache_evict"]
+
+BLOCK = 64  # tokens under one scale
+_E4M3 = torch.float8_e4m3fn
+
+Ints = Union[int, torch.Tensor]
+
+
+class KVCache8:
+    """Keys ``k8`` ``[B, H, capacity, D]`` and values ``v8`` ``[B, H, capacity / 64,
+    D, 64]`` (each block of 64 tokens transposed) in ``float8_e4m3fn``, and the
+    blocks' scales ``k_scale``, ``v_scale`` ``[B, H, capacity / 64]``: fp32 powers of
+    two in [2^-60, 2^60].  Contiguous, D 64 or 128.  How many tokens of it are in
+    use is its user's to say, at every call."""
+
+    __slots__ = ("k8", "v8", "k_scale", "v_scale", "_c")
+
+    def __init__(self, k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        _require_device(k8, v8, k_scale, v_scale)
+        if k8.dim() != 4:
+            raise ValueError(f"k8 must be [B, H, capacity, D], got shape {tuple(k8.shape)}")
+        B, H, n, D = k8.shape
+        if D not in (64, 128) or n < BLOCK or n % BLOCK or B < 1 or H < 1:
+            raise ValueError(f"an 8-bit cache holds head dims 64 and 128 and a multiple of {BLOCK} tokens, "
+                             f"got {tuple(k8.shape)}")
+        if tuple(v8.shape) != (B, H, n // BLOCK, D, BLOCK):
+            raise ValueError(f"v8 must be {(B, H, n // BLOCK, D, BLOCK)}, got {tuple(v8.shape)}")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if tuple(t.shape) != (B, H, n // BLOCK) or t.dtype != torch.float32:
+                raise ValueError(f"{name} must be fp32 {(B, H, n // BLOCK)}, got {t.dtype} {tuple(t.shape)}")
+        if k8.dtype != _E4M3 or v8.dtype != _E4M3:
+            raise ValueError(f"k8 and v8 must be {_E4M3}, got {k8.dtype} and {v8.dtype}")
+        if not all(t.is_contiguous() for t in (k8, v8, k_scale, v_scale)) or k8.data_ptr() % 16 or v8.data_ptr() % 16:
+            raise ValueError("a cache's tensors must be contiguous, k8 and v8 on 16-byte boundaries")
+        self.k8, self.v8, self.k_scale, self.v_scale = k8, v8, k_scale, v_scale
+        self._c = _lib.Cache8(k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, H, n, D)
+
+    @classmethod
+    def empty(cls, batch: int, heads: int, capacity: int, head_dim: int, device=None) -> "KVCache8":
+        """A cache of zeros with room for ``capacity`` tokens (rounded up to a block)."""
+        dev = torch.device("cuda") if device is None else torch.device(device)
+        nb = -(-int(capacity) // BLOCK)
+        return cls(torch.zeros((batch, heads, nb * BLOCK, head_dim), dtype=torch.uint8, device=dev).view(_E4M3),
+                   torch.zeros((batch, heads, nb, head_dim, BLOCK), dtype=torch.uint8, device=dev).view(_E4M3),
+                   torch.ones((batch, heads, nb), dtype=torch.float32, device=dev),
+                   torch.ones((batch, heads, nb), dtype=torch.float32, device=dev))
+
+    @property
+    def shape(self) -> tuple[int, int, int, int]:
+        """(batch, heads, capacity, head_dim)."""
+        return tuple(self.k8.shape)
+
+    @property
+    def capacity(self) -> int:
+        return self.k8.shape[2]
+
+    @property
+    def device(self) -> torch.device:
+        return self.k8.device
+
+    def extended(self, capacity: int, batch: Optional[int] = None) -> "KVCache8":
+        """A copy with room for ``capacity`` tokens; a cache of one item may become
+        one of ``batch`` equal items.  What lies behind this cache's tokens is not
+        initialised."""
+        B, H, n, D = self.shape
+        batch = B if batch is None else int(batch)
+        nb, old = -(-int(capacity) // BLOCK), n // BLOCK
+        if batch != B and B != 1:
+            raise ValueError(f"a cache of {B} items cannot become one of {batch}")
+        if nb < old:
+            raise ValueError(f"capacity {capacity} is below this cache's {n}")
+        parts = []
+        for t, shape in ((self.k8.view(B, H, old, BLOCK, D).view(torch.uint8), (BLOCK, D)),
+                         (self.v8.view(torch.uint8), (D, BLOCK)), (self.k_scale, ()), (self.v_scale, ())):
+            new = torch.empty((batch, H, nb, *shape), dtype=t.dtype, device=t.device)
+            new[:, :, :old] = t
+            parts.append(new)
+        return KVCache8(parts[0].view(_E4M3).view(batch, H, nb * BLOCK, D), parts[1].view(_E4M3), *parts[2:])
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values ``[B, H, capacity, D]`` as numbers."""
+        B, H, n, D = self.shape
+        k = self.k8.float().view(B, H, n // BLOCK, BLOCK, D) * self.k_scale[..., None, None]
+        v = self.v8.float().transpose(-1, -2) * self.v_scale[..., None, None]
+        return k.reshape(B, H, n, D).to(dtype), v.reshape(B, H, n, D).to(dtype)
+
+
+def _ints(x: Ints, name: str, B: int, device: torch.device, lo: int, hi: int) -> torch.Tensor:
+    """``x`` as the int32 ``[B]`` that the kernels read."""
+    if isinstance(x, torch.Tensor):
+        if x.dtype != torch.int32 or tuple(x.shape) != (B,) or x.device != device:
+            raise ValueError(f"{name} must be an int or int32 [{B}] on {device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+        return x.contiguous()
+    x = int(x)
+    if not lo <= x <= hi:
+        raise ValueError(f"{name}={x} must be in [{lo}, {hi}]")
+    return torch.full((B,), x, dtype=torch.int32, device=device)
+
+
+def _no_grad(what: str, *ts: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
+def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start: Ints,
+                 counts: Optional[Ints] = None) -> KVCache8:
+    """Writes ``k``, ``v`` ``[B, H, S, D]`` (fp16, bf16, fp32; any strides) into the
+    cache, in place, from each item's token ``start`` on; of a padded batch the
+    first ``counts`` rows of each item (default: all).
+
+    A block's scale becomes the least power of two that brings the largest of its
+    new rows within 448, and no less than it was where the block keeps rows before
+    ``start`` (those are rounded again if it grows).  To nearest, ties to even;
+    infinities, NaN and magnitudes over 448 * 2^60 become NaN.  Rows that would pass
+    the capacity and items with a negative start are left out; what stood behind
+    the last new row stays.  Returns the cache."""
+    _require_device(cache.k8, k, v)
+    _no_grad("cache_append", k, v)
+    B, H, n, D = cache.shape
+    if k.dim() != 4 or k.shape != v.shape or k.shape[:2] != (B, H) or k.shape[3] != D or k.dtype != v.dtype:
+        raise ValueError(f"k, v must be [{B}, {H}, S, {D}] of one dtype, got {tuple(k.shape)} {k.dtype}, "
+                         f"{tuple(v.shape)} {v.dtype}")
+    S = k.shape[2]
+    code = _dtype_code(k)
+    if S > n:
+        raise ValueError(f"{S} rows for a cache of {n} tokens")
+    if counts is not None:
+        counts = _ints(counts, "counts", B, cache.device, 0, S)
+    start = _ints(start, "start", B, cache.device, 0, n - S)
+    if S == 0:
+        return cache
+    k, ks = rows_of(k, "k")
+    v, vs = rows_of(v, "v")
+    with on_device(k):
+        st = _lib.load().lcv_bsa_cache_append(cache._c, k.data_ptr(), v.data_ptr(), code, S, ks, vs, start.data_ptr(),
+                                              None if counts is None else counts.data_ptr(), _stream(k))
+    _lib.check(st, "cache_append")
+    return cache
+
+
+def _queries(what, q, cache, lengths, q_lens, sm_scale, max_len):
+    """The arguments that attention and its weights share, checked."""
+    _require_device(cache.k8, q)
+    _no_grad(what, q)
+    B, H, n, D = cache.shape
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[1] < H or q.shape[1] % H:
+        raise ValueError(f"q must be [{B}, a multiple of {H}, S, {D}], got {tuple(q.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{what} takes float16 and bfloat16 queries, got {q.dtype}")
+    sm_scale = D ** -0.5 if sm_scale is None else float(sm_scale)
+    if not 0.0 <= sm_scale < math.inf:
+        raise ValueError(f"sm_scale={sm_scale} must be finite and not negative")
+    max_len = n if max_len is None else min(int(max_len), n)
+    if max_len < 0:
+        raise ValueError(f"max_len={max_len} is negative")
+    lengths = _ints(lengths, "lengths", B, cache.device, 0, n)
+    if q_lens is not None:
+        q_lens = _ints(q_lens, "q_lens", B, cache.device, 0, q.shape[2])
+    return lengths, q_lens, sm_scale, max_len
+
+
+def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens: Optional[Ints] = None,
+                     causal: bool = False, sm_scale: Optional[float] = None, max_len: Optional[int] = None,
+                     out: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """``softmax(sm_scale q k^T) v`` of ``q`` ``[B, Hq, S, D]`` (fp16 / bf16, any
+    strides) over the first ``lengths`` tokens of each item's cache; query head h
+    reads key head ``h // (Hq / H)``.
+
+    ``q_lens``: how many of the S queries of each item are real (default: all).
+    ``causal``: the real queries are the item's last tokens, and query i sees the
+    tokens up to ``lengths - q_lens + i``.  Rows that see nothing (padding, empty
+    items, queries before the first token) get zeros.  ``max_len``: a bound on
+    ``lengths`` known to the caller (longer items count as that long); it shapes the
+    launch, so a close one serves short histories in a long cache.
+
+    Returns ``out`` ``[B, Hq, S, D]`` in q's dtype, or ``(out, lse)`` with the fp32
+    ``[B, Hq, S]`` log of each row's sum (-inf where nothing is seen)."""
+    lengths, q_lens, sm_scale, max_len = _queries("cached_attention", q, cache, lengths, q_lens, sm_scale, max_len)
+    B, Hq, S, D = q.shape
+    if out is None:
+        out = torch.empty((B, Hq, S, D), dtype=q.dtype, device=q.device)
+    else:
+        _require_device(q, out)
+        _no_grad("cached_attention", out)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
+        if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+            raise ValueError("out's elements share memory")
+    lse = torch.empty((B, Hq, S), dtype=torch.float32, device=q.device) if return_lse else None
+    if q.numel() == 0 or max_len == 0:
+        out.zero_()
+        if return_lse:
+            lse.fill_(-math.inf)
+        return (out, lse) if return_lse else out
+    q, qs = rows_of(q, "q")
+    to, os = rows_of(out, "out")  # a copy where out's rows cannot be written in place
+    lib = _lib.load()
+    size = lib.lcv_bsa_cached_attn_workspace_bytes(Hq, S, cache._c, max_len)
+    ws = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
+    with on_device(q):
+        st = lib.lcv_bsa_cached_attn(q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._c, lengths.data_ptr(),
+                                     None if q_lens is None else q_lens.data_ptr(), int(causal), sm_scale, max_len,
+                                     to.data_ptr(), os, None if lse is None else lse.data_ptr(),
+                                     None if ws is None else ws.data_ptr(), size, _stream(q))
+    _lib.check(st, "cached_attention")
+    if to is not out:
+        out.copy_(to)
+    return (out, lse) if return_lse else out
+
+
+def attention_weights(q: torch.Tensor, cache: KVCache8, lengths: Ints, lse: torch.Tensor, *,
+                      q_lens: Optional[Ints] = None, causal: bool = False, sm_scale: Optional[float] = None,
+                      max_len: Optional[int] = None, weights: Optional[torch.Tensor] = None,
+                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``weights`` (fp32 ``[B, H, capacity]``; default zeros) plus, for each cached
+    token, the attention that these queries gave it: the sum of their softmax over
+    the rows of its key head.  ``lse`` and the other arguments are those of
+    ``cached_attention``.  ``out`` may be ``weights`` itself, to accumulate in place.
+    The same call gives the same bits."""
+    lengths, q_lens, sm_scale, max_len = _queries("attention_weights", q, cache, lengths, q_lens, sm_scale, max_len)
+    B, Hq, S, D = q.shape
+    shape = (B, cache.shape[1], cache.capacity)
+    if tuple(lse.shape) != (B, Hq, S) or lse.dtype != torch.float32:
+        raise ValueError(f"lse must be fp32 {(B, Hq, S)}, got {lse.dtype} {tuple(lse.shape)}")
+    for name, t in (("weights", weights), ("out", out)):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float32):
+            raise ValueError(f"{name} must be fp32 {shape}, got {t.dtype} {tuple(t.shape)}")
+    _require_device(q, lse, *(t for t in (weights, out) if t is not None))
+    _no_grad("attention_weights", lse, *(t for t in (weights, out) if t is not None))
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=q.device)
+    elif not out.is_contiguous():
+        raise ValueError("out must be contiguous")
+    if q.numel() == 0 or max_len == 0:
+        return out.zero_() if weights is None else out.copy_(weights) if out is not weights else out
+    q, qs = rows_of(q, "q")
+    lse = lse.contiguous()
+    weights = None if weights is None else weights.contiguous()
+    with on_device(q):
+        st = _lib.load().lcv_bsa_attention_weights(
+            q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._c, lengths.data_ptr(),
+            None if q_lens is None else q_lens.data_ptr(), int(causal), sm_scale, max_len, lse.data_ptr(),
+            None if weights is None else weights.data_ptr(), out.data_ptr(), _stream(q))
+    _lib.check(st, "attention_weights")
+    return out
+
+
+def cache_evict(cache: KVCache8, lengths: Ints, weights: torch.Tensor, keep: int, *, recent: int = 0):
+    """Of each head's ``lengths`` tokens, the newest ``recent`` and the heaviest others
+    (by ``weights`` ``[B, H, capacity]`` fp32; equal ones: the lowest token first; NaN
+    below everything), ``keep`` in all, in their order, as a new cache.
+
+    Returns ``(cache, weights, kept, lengths)``: the new cache (capacity ``keep``
+    rounded up to a block, each block under the least scale for its rows, zeros
+    behind the last), the kept tokens' weights (zeros behind), their old indices
+    ``[B, H, keep]`` int32 (-1 behind) and the new lengths ``[B]`` int32."""
+    _require_device(cache.k8, weights)
+    _no_grad("cache_evict", weights)
+    B, H, n, D = cache.shape
+    if tuple(weights.shape) != (B, H, n) or weights.dtype != torch.float32:
+        raise ValueError(f"weights must be fp32 {(B, H, n)}, got {weights.dtype} {tuple(weights.shape)}")
+    keep, recent = int(keep), int(recent)
+    if keep < 1 or not 0 <= recent <= keep:
+        raise ValueError(f"keep={keep} must be at least 1 and recent={recent} in [0, keep]")
+    lengths = _ints(lengths, "lengths", B, cache.device, 0, n)
+    weights = weights.contiguous()
+    dev, nb = cache.device, -(-keep // BLOCK)
+    new = KVCache8(torch.empty((B, H, nb * BLOCK, D), dtype=_E4M3, device=dev),
+                   torch.empty((B, H, nb, D, BLOCK), dtype=_E4M3, device=dev),
+                   torch.empty((B, H, nb), dtype=torch.float32, device=dev),
+                   torch.empty((B, H, nb), dtype=torch.float32, device=dev))
+    new_weights = torch.empty((B, H, nb * BLOCK), dtype=torch.float32, device=dev)
+    kept = torch.empty((B, H, keep), dtype=torch.int32, device=dev)
+    left = torch.empty((B,), dtype=torch.int32, device=dev)
+    with on_device(weights):
+        st = _lib.load().lcv_bsa_cache_evict(cache._c, lengths.data_ptr(), weights.data_ptr(), keep, recent, new._c,
+                                             new_weights.data_ptr(), kept.data_ptr(), left.data_ptr(), _stream(weights))
+    _lib.check(st, "cache_evict")
+    return new, new_weights, kept, left
