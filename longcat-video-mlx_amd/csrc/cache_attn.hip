@@ -12,14 +12,24 @@
 // P' below 2^-14 loses bits only where the block with the larger values has an e4m3
 // step 2^16 times what is lost); sums, maxima and O stay in fp32.
 //
-// The rows of one key head are its group's queries, row r = query r % S of head
-// r / S; a row sees the first `vis` tokens.  What a row does not see has P' = 0, and
+// The rows of one key head are its group's queries, row r = query r / group of the
+// group's head r % group; a row sees the first `vis` tokens, rows in order no fewer.  What a row does not see has P' = 0, and
 // a NaN among the values of such tokens is taken out of its product.
 #include "attn_common.h"
 #include "cache_common.h"
 
 namespace lcv {
 namespace {
+
+// dma16 where the descriptor may have been brought back from spilled lanes right
+// before: a vector instruction's scalar result needs five wait states until a buffer
+// load reads it, and the compiler does not see the load inside the asm.
+__device__ __forceinline__ void dma16_settled(__amdgpu_buffer_rsrc_t rsrc, uint32_t voffset, int32_t soffset,
+                                              uint32_t m0v) {
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+               ::"v"(voffset), "s"(rsrc), "s"(soffset), "{m0}"(m0v)
+               : "memory");
+}
 
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLn2 = 0.69314718055994531f;
@@ -43,240 +53,757 @@ __device__ __forceinline__ int visible(const CacheAttn& a, const Lens& n, int i)
   return v < 0 ? 0 : v;
 }
 
-struct Few {
-  int32_t tiles, splits;
-  float* part_o;   // [work id][16][D]
-  float* part_ml;  // [work id][16][2]
-};
-
-// The 16 rows of a tile, merged from `n` parts (strides in floats), and written.
-template <typename T, int D>
-__device__ __forceinline__ void merge_rows(const CacheAttn& a, int b, int kvh, int tile, const float* o, int64_t o_step,
-                                           const float* ml, int64_t ml_step, int n, float* to_o, float* to_ml) {
-  const int row = threadIdx.x / 16, d0 = threadIdx.x % 16 * (D / 16);
-  float m = kNegInf;
-  for (int i = 0; i < n; ++i) m = __builtin_elementwise_maximum(m, ml[i * ml_step + 2 * row]);
-  const float base = m == kNegInf ? 0.0f : m;
-  float l = 0.0f, acc[D / 16];
-#pragma unroll
-  for (int e = 0; e < D / 16; ++e) acc[e] = 0.0f;
-  for (int i = 0; i < n; ++i) {
-    const float f = fast_exp2(ml[i * ml_step + 2 * row] - base);
-    l = __builtin_fmaf(ml[i * ml_step + 2 * row + 1], f, l);
-    const float* src = o + i * o_step + row * D + d0;
-#pragma unroll
-    for (int e = 0; e < D / 16; ++e) acc[e] = __builtin_fmaf(src[e], f, acc[e]);
-  }
-  if (to_o) {
-#pragma unroll
-    for (int e = 0; e < D / 16; ++e) to_o[row * D + d0 + e] = acc[e];
-    if (d0 == 0) {
-      to_ml[2 * row] = m;
-      to_ml[2 * row + 1] = l;
-    }
-    return;
-  }
-  const int r = tile * 16 + row;
-  if (r >= a.group * a.S) return;
-  const int g = r / a.S, i = r - g * a.S;
-  const int h = kvh * a.group + g;
-  const bool empty = m == kNegInf;
-  const float inv = 1.0f / l;
-  T* out = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + (int64_t)b * a.out.sb + (int64_t)h * a.out.sh +
-           (int64_t)i * a.out.ss + d0;
-  T t[D / 16];
-#pragma unroll
-  for (int e = 0; e < D / 16; ++e) t[e] = from_f32<T>(empty ? 0.0f : acc[e] * inv);
-  __builtin_memcpy(__builtin_assume_aligned(out, 2 * D / 16), t, sizeof(t));
-  if (a.lse && d0 == 0)
-    a.lse[((int64_t)b * a.c.H * a.group + h) * a.S + i] = empty ? kNegInf : (m + __builtin_log2f(l)) * kLn2;
+// Keeps what follows from being computed before the branch that it stands in.
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
-// Few rows: one workgroup walks a part of one key head's blocks for 16 rows, its
-// four waves taking every fourth block.  The operands come straight from memory in
-// the layout the products want (16 x 16 x 32 MFMAs, P in registers): lane (G, gi) =
-// (lane / 16, lane % 16) holds, of key tile t of a block, key 16 (gi / 4) + 4 t + gi % 4
-// at D/4 contiguous values from G D / 4, so that the scores' accumulators hold keys
-// 16 G + 4 t + i of row gi, which is the order of the 16 bytes that a lane reads of
-// v8's row 16 dt + gi.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void few_rows_kernel(CacheAttn a, Few f) {
+// What the rows [r0, r1) of a key head see: the most of any, and the least of those that
+// see any token.
+struct Reach {
+  int most, least;
+};
+__device__ __forceinline__ Reach reach(const CacheAttn& a, const Lens& n, int r0, int r1) {
+  const int rows = a.group * a.S;
+  if (r1 > rows) r1 = rows;
+  const int i0 = r0 / a.group;
+  if (r0 >= r1 || i0 >= n.ql) return {0, 0};
+  int i1 = (r1 - 1) / a.group;
+  if (i1 >= n.ql) i1 = n.ql - 1;
+  const int least = visible(a, n, i0);
+  return {visible(a, n, i1), least > 0 ? least : 1};
+}
+
+// How the walk over the blocks is split: parts of `per` blocks, at most `splits`.  Their
+// sums and maxima lie in the workspace by (split, key head, 16 rows).
+struct Parts {
+  int32_t tiles;   // of 16 rows, of one key head
+  int32_t splits, per;
+  float* o;        // [splits][B * H][tiles][16][D]
+  float* ml;       // [splits][B * H][tiles][16][2]
+};
+__device__ __forceinline__ int64_t part_at(const CacheAttn& a, const Parts& p, int split, int bh, int tile) {
+  return ((int64_t)split * a.c.B * a.c.H + bh) * p.tiles + tile;
+}
+
+template <typename T>
+__device__ __forceinline__ T* out_row(const CacheAttn& a, int b, int kvh, int r) {
+  return reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + (int64_t)b * a.out.sb +
+         (int64_t)(kvh * a.group + r % a.group) * a.out.sh + (int64_t)(r / a.group) * a.out.ss;
+}
+template <typename T>
+__device__ __forceinline__ const T* q_row(const CacheAttn& a, int b, int kvh, int r) {
+  return reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb + (int64_t)(kvh * a.group + r % a.group) * a.q.sh +
+         (int64_t)(r / a.group) * a.q.ss;
+}
+__device__ __forceinline__ int64_t lse_at(const CacheAttn& a, int b, int kvh, int r) {
+  return ((int64_t)b * a.c.H * a.group + kvh * a.group + r % a.group) * a.S + r / a.group;
+}
+
+// Few rows: one workgroup walks a part of one key head's blocks for 16 or 32 rows (NT
+// tiles), its four waves taking every fourth block.  The operands come straight from
+// memory in the layout the products want (16 x 16 x 32 MFMAs, P in registers): lane
+// (G, gi) = (lane / 16, lane % 16) holds, of key tile t of a block, key
+// 16 (gi / 4) + 4 t + gi % 4 at D/4 contiguous values from G D / 4, so that the scores'
+// accumulators hold keys 16 G + 4 t + i of row gi, which is the order of the 16 bytes
+// that a lane reads of v8's row 16 dt + gi.  Keys and values of a wave's next block are
+// asked for as soon as those of this one are used.
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, NT == 1 ? 3 : 2)))
+void few_rows_kernel(CacheAttn a, Parts p) {
   typedef typename Mfma<T>::vec8 vec8;
   __shared__ float part_o[4][16 * D];
   __shared__ float part_ml[4][32];
-  const int wid = xcd_linear_work_id(blockIdx.x, gridDim.x);
-  const int tile = wid % f.tiles;
-  const int split = wid / f.tiles % f.splits;
-  const int bh = wid / (f.tiles * f.splits);
+  // Work: (part, key head) u, whose tiles follow one another on one XCD (u % 8); heads
+  // next to one another, so that every XCD has some of every item's.
+  const int heads = a.c.B * a.c.H, slot = blockIdx.x / kNumXcd, wide = p.tiles / NT;
+  const int tile = slot % wide * NT;
+  const int u = slot / wide * kNumXcd + blockIdx.x % kNumXcd;
+  const int bh = u % heads, split = u / heads;
+  if (split >= p.splits) return;
   const int b = bh / a.c.H, kvh = bh - b * a.c.H;
   const int lane = threadIdx.x % 64, G = lane / 16, gi = lane % 16;
   const int wave = uniform_i32(threadIdx.x / 64);
   const Lens n = item_lens(a, b);
   const int rows = a.group * a.S;
-  int r = tile * 16 + gi;
-  const int vis = r < rows ? visible(a, n, r % a.S) : 0;
-  r = r < rows ? r : 0;
-  int most = vis;
-  for (int o = 1; o < 16; o <<= 1) {
-    const int x = __shfl_xor(most, o);
-    most = x > most ? x : most;
-  }
-  most = uniform_i32(most);
-  const int nblk = (most + 63) / 64;
-  const int j0 = (int)((int64_t)split * nblk / f.splits), j1 = (int)((int64_t)(split + 1) * nblk / f.splits);
+  const Reach all = reach(a, n, 16 * tile, 16 * tile + 16 * NT);
+  const int nblk = (all.most + 63) / 64;
+  const int j0 = split * p.per;
+  const int j1 = j0 + p.per < nblk ? j0 + p.per : nblk;
+  if (split > 0 && j0 >= nblk) return;  // the first part of a tile always answers
 
-  const T* q = reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb +
-               (int64_t)(kvh * a.group + r / a.S) * a.q.sh + (int64_t)(r % a.S) * a.q.ss + G * (D / 4);
-  vec8 qf[D / 32];
+  vec8 qf[NT][D / 32];
+  int vis[NT];
 #pragma unroll
-  for (int ks = 0; ks < D / 32; ++ks)
-    qf[ks] = __builtin_bit_cast(vec8, *reinterpret_cast<const u32x4*>(q + 8 * ks));
-
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = 16 * (tile + nt) + gi;
+    vis[nt] = r < rows ? visible(a, n, r / a.group) : 0;
+    const T* q = q_row<T>(a, b, kvh, r < rows ? r : 0) + G * (D / 4);
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks)
+      qf[nt][ks] = __builtin_bit_cast(vec8, *reinterpret_cast<const u32x4*>(q + 8 * ks));
+  }
   const uint8_t* kb = a.c.k8 + (int64_t)bh * a.c.nb * (64 * D) + (16 * (gi / 4) + gi % 4) * D + G * (D / 4);
   const uint8_t* vb = a.c.v8 + (int64_t)bh * a.c.nb * (64 * D) + gi * 64 + 16 * G;
   const float* ksc = a.c.k_scale + (int64_t)bh * a.c.nb;
   const float* vsc = a.c.v_scale + (int64_t)bh * a.c.nb;
 
-  f32x4 o[D / 16];
+  f32x4 o[NT][D / 16];
+  float m[NT], l[NT];
 #pragma unroll
-  for (int dt = 0; dt < D / 16; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = kNegInf, l = 0.0f;
-  for (int j = j0 + wave; j < j1; j += 4) {
-    u32x4 kw[4][D / 64], vw[D / 16];
-    const uint8_t* kj = kb + (int64_t)j * (64 * D);
-    const uint8_t* vj = vb + (int64_t)j * (64 * D);
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt] = kNegInf, l[nt] = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int dt = 0; dt < D / 16; ++dt) o[nt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  u32x4 kw[4][D / 64], vw[D / 16];
+  float ks_next = 0.0f, vs_next = 0.0f;
+  auto ask_k = [&](int j, int t) {
 #pragma unroll
-      for (int u = 0; u < D / 64; ++u) kw[t][u] = *reinterpret_cast<const u32x4*>(kj + 4 * t * D + 16 * u);
+    for (int u = 0; u < D / 64; ++u)
+      kw[t][u] = *reinterpret_cast<const u32x4*>(kb + (int64_t)j * (64 * D) + 4 * t * D + 16 * u);
+  };
+  auto ask_v = [&](int j, int dt) {
+    vw[dt] = *reinterpret_cast<const u32x4*>(vb + (int64_t)j * (64 * D) + dt * (16 * 64));
+  };
+  auto ask_scales = [&](int j) { ks_next = ksc[j], vs_next = vsc[j]; };
+  int j = j0 + wave;
+  if (j < j1) {
+    ask_scales(j);
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) vw[dt] = *reinterpret_cast<const u32x4*>(vj + dt * (16 * 64));
-    const float c = a.scale_log2 * ksc[j];
-    const int ev = exponent_of(vsc[j]);
-    f32x4 s[4];
+    for (int t = 0; t < 4; ++t) ask_k(j, t);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) ask_v(j, dt);
+  }
+  for (; j < j1; j += 4) {
+    const int jn = j + 4 < j1 ? j + 4 : j;  // past the end: this block again, unused
+    const float c = a.scale_log2 * ks_next > 0x1p-126f ? a.scale_log2 * ks_next : 0x1p-126f;
+    const int ev = exponent_of(vs_next);
+    f32x4 s[NT][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int ks = 0; ks < D / 32; ++ks)
-        s[t] = Mfma<T>::mma(From8<T>::cvt(kw[t][ks / 2][2 * (ks % 2)], kw[t][ks / 2][2 * (ks % 2) + 1]), qf[ks], s[t]);
+      for (int nt = 0; nt < NT; ++nt) s[nt][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int ks = 0; ks < D / 32; ++ks) {
+        const vec8 k = From8<T>::cvt(kw[t][ks / 2][2 * (ks % 2)], kw[t][ks / 2][2 * (ks % 2) + 1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[nt][t] = Mfma<T>::mma(k, qf[nt][ks], s[nt][t]);
+      }
     }
-    const int left = vis - 64 * j - 16 * G;  // key 4 t + i of this lane is seen if below
-    float mx = kNegInf;
+    ask_scales(jn);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[t][i] = 4 * t + i < left ? s[t][i] * c : kNegInf;
-        mx = __builtin_elementwise_maximum(mx, s[t][i]);
-      }
-    mx = max_quarters(mx);
+    for (int t = 0; t < 4; ++t) ask_k(jn, t);
+    const bool part = 64 * j + 64 > all.least;  // some row sees the block in part
+    vec8 pf[NT][2];
+    float down[NT];
     const float fev = (float)ev;
-    const float m_new = __builtin_elementwise_maximum(m, mx + fev);
-    const float base = m_new == kNegInf ? 0.0f : m_new;
-    const float down = fast_exp2(m - base);
-    const float off = fev - base;
-    vec8 pf[2];
-    float sum = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int nt = 0; nt < NT; ++nt) {
+      if (part) {
+        const int left = here(vis[nt] - 64 * j - 16 * G);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = fast_exp2(s[t][i] + off);
-        sum += p;
-        pf[t / 2][4 * (t % 2) + i] = from_f32<T>(p);
+        for (int x = 0; x < 16; ++x)
+          if (x >= left) s[nt][x / 4][x % 4] = kNegInf;
       }
-    l = __builtin_fmaf(l, down, sum * pow2i(-ev));
-    m = m_new;
-    // A block that some row sees in part: NaN bytes count for the rows that see them alone.
+      float mx = s[nt][0][0];
+#pragma unroll
+      for (int x = 1; x < 16; ++x) mx = __builtin_elementwise_maximum(mx, s[nt][x / 4][x % 4]);
+      const float m_new = __builtin_elementwise_maximum(m[nt], __builtin_fmaf(max_quarters(mx), c, fev));
+      const float base = m_new == kNegInf ? 0.0f : m_new;
+      down[nt] = fast_exp2(m[nt] - base);
+      const float off = fev - base;
+      float sum = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const float e = fast_exp2(__builtin_fmaf(s[nt][x / 4][x % 4], c, off));
+        sum += e;
+        pf[nt][x / 8][x % 8] = from_f32<T>(e);
+      }
+      l[nt] = __builtin_fmaf(l[nt], down[nt], sum * pow2i(-ev));
+      m[nt] = m_new;
+    }
+    // NaN bytes of a block that some row sees in part count for the rows that see them alone.
     uint32_t bad = 0;
-    if (__ballot(vis > 0 && vis < 64 * j + 64)) {
+    if (part) {
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) bad |= nan_bytes(vw[dt][e]);
     }
     if (__ballot(bad != 0)) {
-      vec8 seen[2];
+      vec8 seen[NT][2];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) seen[e / 8][e % 8] = from_f32<T>(e < left ? 1.0f : 0.0f);
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          seen[nt][x / 8][x % 8] = from_f32<T>(64 * j + 16 * G + x < vis[nt] ? 1.0f : 0.0f);
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) {
         u32x4 is;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t nan = nan_bytes(vw[dt][e]);
-          is[e] = nan >> 7 << 3;                        // 0x08: a positive number
-          vw[dt][e] &= ~((nan - (nan >> 7)) | nan);     // zero
+          is[e] = nan >> 7 << 3;                     // a positive number for each
+          vw[dt][e] &= ~((nan - (nan >> 7)) | nan);  // zero
         }
-        f32x4 hit = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const vec8 i0 = From8<T>::cvt(is[0], is[1]), i1 = From8<T>::cvt(is[2], is[3]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) hit = Mfma<T>::mma(From8<T>::cvt(is[2 * u], is[2 * u + 1]), seen[u], hit);
+        for (int nt = 0; nt < NT; ++nt) {
+          f32x4 hit = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          hit = Mfma<T>::mma(i0, seen[nt][0], hit);
+          hit = Mfma<T>::mma(i1, seen[nt][1], hit);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (hit[i] > 0.0f) o[dt][i] = __builtin_nanf("");
+          for (int i = 0; i < 4; ++i)
+            if (hit[i] > 0.0f) o[nt][dt][i] = __builtin_nanf("");
+        }
       }
     }
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
+      const vec8 v0 = From8<T>::cvt(vw[dt][0], vw[dt][1]), v1 = From8<T>::cvt(vw[dt][2], vw[dt][3]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[dt][i] *= down;
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        o[dt] = Mfma<T>::mma(From8<T>::cvt(vw[dt][2 * u], vw[dt][2 * u + 1]), pf[u], o[dt]);
+        for (int i = 0; i < 4; ++i) o[nt][dt][i] *= down[nt];
+        o[nt][dt] = Mfma<T>::mma(v0, pf[nt][0], o[nt][dt]);
+        o[nt][dt] = Mfma<T>::mma(v1, pf[nt][1], o[nt][dt]);
+      }
+      ask_v(jn, dt);
     }
   }
-  l = sum_quarters(l);
+  // The four waves' parts together: thread (row, 16th of D).
+  const bool last = nblk <= p.per;  // nothing to join
+  const int row = threadIdx.x / 16, d0 = threadIdx.x % 16 * (D / 16);
 #pragma unroll
-  for (int dt = 0; dt < D / 16; ++dt)
-    *reinterpret_cast<f32x4*>(&part_o[wave][gi * D + 16 * dt + 4 * G]) = o[dt];
-  if (G == 0) {
-    part_ml[wave][2 * gi] = m;
-    part_ml[wave][2 * gi + 1] = l;
+  for (int nt = 0; nt < NT; ++nt) {
+    const float sum = sum_quarters(l[nt]);
+    __syncthreads();
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+      *reinterpret_cast<f32x4*>(&part_o[wave][gi * D + 16 * dt + 4 * G]) = o[nt][dt];
+    if (G == 0) {
+      part_ml[wave][2 * gi] = m[nt];
+      part_ml[wave][2 * gi + 1] = sum;
+    }
+    __syncthreads();
+    const int r = 16 * (tile + nt) + row;
+    if (r >= rows) continue;
+    float top = kNegInf;
+    for (int w = 0; w < 4; ++w) top = __builtin_elementwise_maximum(top, part_ml[w][2 * row]);
+    const float base = top == kNegInf ? 0.0f : top;
+    float lsum = 0.0f, acc[D / 16];
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) acc[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = fast_exp2(part_ml[w][2 * row] - base);
+      lsum = __builtin_fmaf(part_ml[w][2 * row + 1], f, lsum);
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) acc[e] = __builtin_fmaf(part_o[w][row * D + d0 + e], f, acc[e]);
+    }
+    if (last) {
+      const bool empty = top == kNegInf || visible(a, n, r / a.group) == 0;
+      const float inv = 1.0f / lsum;
+      T t[D / 16];
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) t[e] = from_f32<T>(empty ? 0.0f : acc[e] * inv);
+      __builtin_memcpy(__builtin_assume_aligned(out_row<T>(a, b, kvh, r) + d0, 2 * D / 16), t, sizeof(t));
+      if (a.lse && d0 == 0) a.lse[lse_at(a, b, kvh, r)] = empty ? kNegInf : (top + __builtin_log2f(lsum)) * kLn2;
+    } else {
+      const int64_t at = part_at(a, p, split, bh, tile + nt);
+      __builtin_memcpy(__builtin_assume_aligned(p.o + at * (16 * D) + row * D + d0, 4 * D / 16), acc, sizeof(acc));
+      if (d0 == 0) {
+        p.ml[at * 32 + 2 * row] = top;
+        p.ml[at * 32 + 2 * row + 1] = lsum;
+      }
+    }
   }
-  __syncthreads();
-  merge_rows<T, D>(a, b, kvh, tile, part_o[0], 16 * D, part_ml[0], 32, 4,
-                   f.splits > 1 ? f.part_o + (int64_t)wid * (16 * D) : nullptr, f.part_ml + (int64_t)wid * 32);
 }
+
+// A row's parts together.  `wide` rows share a walk, whose reach says how many parts there
+// are.  THREADS threads take a row: a wave where there are few rows, so that many loads
+// are under way, 16 where there are many.
+template <typename T, int D, int THREADS>
+__global__ __launch_bounds__(256) void join_kernel(CacheAttn a, Parts p, int wide, int64_t total) {
+  constexpr int kN = D / THREADS;
+  const int64_t id = (int64_t)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
+  if (id >= total) return;
+  const int rows = a.group * a.S;
+  const int r = (int)(id % rows), bh = (int)(id / rows);
+  const int b = bh / a.c.H, kvh = bh - b * a.c.H;
+  const Lens n = item_lens(a, b);
+  const int first = r / wide * wide;
+  const int nblk = (reach(a, n, first, first + wide).most + 63) / 64;
+  if (nblk <= p.per) return;  // written already
+  const int parts = (nblk + p.per - 1) / p.per;
+  const int lane = threadIdx.x % THREADS;
+  const int64_t step = (int64_t)a.c.B * a.c.H * p.tiles;
+  const int64_t at = part_at(a, p, 0, bh, r / 16);
+  const float* ml = p.ml + at * 32 + 2 * (r % 16);
+  const float* o = p.o + at * (16 * D) + r % 16 * D + lane * kN;
+  float top = kNegInf;
+  for (int i = lane; i < parts; i += THREADS) top = __builtin_elementwise_maximum(top, ml[i * step * 32]);
+  for (int x = 1; x < THREADS; x <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, x));
+  const float base = top == kNegInf ? 0.0f : top;
+  float lsum = 0.0f, acc[kN];
+#pragma unroll
+  for (int e = 0; e < kN; ++e) acc[e] = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const float f = fast_exp2(ml[i * step * 32] - base);
+    lsum = __builtin_fmaf(ml[i * step * 32 + 1], f, lsum);
+    float x[kN];
+    __builtin_memcpy(x, __builtin_assume_aligned(o + i * step * (16 * D), 4 * kN > 16 ? 16 : 4 * kN), sizeof(x));
+#pragma unroll
+    for (int e = 0; e < kN; ++e) acc[e] = __builtin_fmaf(x[e], f, acc[e]);
+  }
+  const bool empty = top == kNegInf || visible(a, n, r / a.group) == 0;
+  const float inv = 1.0f / lsum;
+  T t[kN];
+#pragma unroll
+  for (int e = 0; e < kN; ++e) t[e] = from_f32<T>(empty ? 0.0f : acc[e] * inv);
+  __builtin_memcpy(__builtin_assume_aligned(out_row<T>(a, b, kvh, r) + lane * kN, 2 * kN), t, sizeof(t));
+  if (a.lse && lane == 0) a.lse[lse_at(a, b, kvh, r)] = empty ? kNegInf : (top + __builtin_log2f(lsum)) * kLn2;
+}
+
+// Many rows: one workgroup of four waves takes 128 rows of one key head, wave w rows
+// 32 w .. 32 w + 31, and walks a part of the blocks.  A block's 8 KB of keys and 8 KB
+// of values (D = 128) go straight from memory into a ring of three LDS slots, two
+// blocks ahead, one barrier a block; every wave turns the bytes into T as it reads
+// them.  Operands as in few_rows_kernel.  LDS rows are 64 or 128 bytes in chunks of 16,
+// chunk c of row r at c ^ swz(r), so that the 16 rows that a lane group reads at once
+// lie in different banks.
+//
+// A row's offset m is the maximum of its first half block, and later halves need no
+// maximum; their P' may pass 1.  Where a half's sum passes a bound (2^15 in fp16, whose
+// range ends there; 2^40 in bf16), or is NaN, the workgroup walks again with the rows'
+// exact maxima.  (Rescaling O inside the walk costs it 60 registers.)
+template <typename T>
+constexpr float kMaxSum = 0x1p40f;
+template <>
+constexpr float kMaxSum<f16> = 0x1p15f;
+
+template <int D>
+struct Tile8 {
+  static constexpr int kKeyChunks = D / 16;  // of a key's row
+  __device__ static int kswz(int r) { return D == 128 ? ((r >> 4) << 1 | ((r >> 1) & 1)) : r >> 4; }
+  __device__ static int vswz(int d) { return (d >> 2) & 3; }
+};
+
+template <bool B>
+struct Flag {
+  static constexpr bool value = B;
+};
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void join_kernel(CacheAttn a, Few f) {
-  const int tile = blockIdx.x % f.tiles, bh = blockIdx.x / f.tiles;
-  const int64_t first = (int64_t)bh * f.tiles * f.splits + tile;
-  merge_rows<T, D>(a, bh / a.c.H, bh % a.c.H, tile, f.part_o + first * (16 * D), (int64_t)f.tiles * (16 * D),
-                   f.part_ml + first * 32, (int64_t)f.tiles * 32, f.splits, nullptr, nullptr);
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 3 : 4, D == 128 ? 3 : 4)))
+void many_rows_kernel(CacheAttn a, Parts p) {
+  typedef typename Mfma<T>::vec8 vec8;
+  typedef Tile8<D> C;
+  constexpr int kHalf = 64 * D;      // bytes of a block's keys or values
+  constexpr int kSlot = 2 * kHalf;
+  constexpr int kLoads = kHalf / 4096;  // 1 KB loads of a wave for keys, and for values
+  constexpr int kRows = 128;
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[3 * kSlot];
+  static_assert(3 * kSlot >= kRows * 2 * D, "the ring stages the output rows");
+
+  // Work ids: batch items next to one another, then the tiles of a head, its parts, the
+  // heads.  Items of different lengths then share an XCD's time.
+  const int wid = xcd_linear_work_id(blockIdx.x, gridDim.x);
+  const int turn = wid / a.c.B * a.c.B / 32;  // a CU's workgroups, 32 apart, are not all one item's
+  const int b = (wid % a.c.B + turn) % a.c.B;
+  const int tiles = p.tiles / 8;  // of 128 rows
+  const int at = wid / a.c.B % tiles;
+  const int tile = a.causal ? tiles - 1 - at : at;  // the longest walks first
+  const int split = wid / (a.c.B * tiles) % p.splits;
+  const int kvh = wid / (a.c.B * tiles * p.splits);
+  const int bh = b * a.c.H + kvh;
+  const int tid = threadIdx.x, lane = tid % 64, G = lane / 16, gi = lane % 16;
+  const int wave = uniform_i32(tid / 64);
+  const Lens n = item_lens(a, b);
+  const int rows = a.group * a.S;
+  const int nblk = (reach(a, n, kRows * tile, kRows * tile + kRows).most + 63) / 64;
+  const int j0 = split * p.per;
+  const int j1 = j0 + p.per < nblk ? j0 + p.per : nblk;
+  if (split > 0 && j0 >= nblk) return;  // the first part of a tile always answers
+  const Reach mine = reach(a, n, kRows * tile + 32 * wave, kRows * tile + 32 * wave + 32);
+  const int own = uniform_i32(mine.most), least = uniform_i32(mine.least);
+
+  int vis[2];
+  vec8 qf[2][D / 32];
+#pragma unroll
+  for (int qt = 0; qt < 2; ++qt) {
+    const int r = kRows * tile + 32 * wave + 16 * qt + gi;
+    vis[qt] = r < rows ? visible(a, n, r / a.group) : 0;
+    const T* q = q_row<T>(a, b, kvh, r < rows ? r : 0) + G * (D / 4);
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks)  // a row that sees nothing: no number of its own gets into a sum
+      qf[qt][ks] = __builtin_bit_cast(
+          vec8, vis[qt] > 0 ? *reinterpret_cast<const u32x4*>(q + 8 * ks) : u32x4{0u, 0u, 0u, 0u});
+  }
+  __shared__ int wave_dirty[4];
+
+  const uint32_t head_bytes = (uint32_t)a.c.nb * (uint32_t)kHalf;  // capacities are limited so that this fits
+  const uint8_t* vhead = a.c.v8 + (int64_t)bh * a.c.nb * kHalf;
+  const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
+      a.c.k8 + (int64_t)bh * a.c.nb * kHalf, (short)0, (int)head_bytes, kBufferFlags);
+  const __amdgpu_buffer_rsrc_t vrs =
+      __builtin_amdgcn_make_buffer_rsrc((void*)vhead, (short)0, (int)head_bytes, kBufferFlags);
+  uint32_t ko[kLoads], vo[kLoads];
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u) {
+    const int slot = 64 * (kLoads * wave + u) + lane;  // 16-byte chunk of the block
+    const int kr = slot / C::kKeyChunks, kc = slot % C::kKeyChunks;
+    ko[u] = 16u * (uint32_t)(kr * C::kKeyChunks + (kc ^ C::kswz(kr)));
+    const int vr = slot / 4, vc = slot % 4;
+    vo[u] = 16u * (uint32_t)(vr * 4 + (vc ^ C::vswz(vr)));
+  }
+  auto fetch = [&](int j, int slot) {
+    const uint32_t m0 = lds_addr(ring + slot * kSlot + 1024 * (kLoads * wave));
+    const int off = (int)((uint32_t)j * (uint32_t)kHalf);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) dma16_settled(krs, ko[u], off, m0 + 1024u * u);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) dma16_settled(vrs, vo[u], off, m0 + kHalf + 1024u * u);
+  };
+
+  // The scales of 64 blocks at a time: lane l holds block base + l's.
+  const float* ksc = a.c.k_scale + (int64_t)bh * a.c.nb;
+  const float* vsc = a.c.v_scale + (int64_t)bh * a.c.nb;
+  float ks64 = 0.0f, vs64 = 0.0f;
+  auto scales = [&](int base) {
+    const int j = base + lane < a.c.nb ? base + lane : a.c.nb - 1;
+    ks64 = ksc[j];
+    vs64 = vsc[j];
+  };
+
+  // A block's keys go in two halves: half h of lane group G is keys 16 G + 8 (h ^ G % 2)
+  // .. + 7 (the groups alternate, so that the 8 bytes that a half reads of each of v8's
+  // chunks lie in all banks), two key tiles of 4 a group.
+  const int hk = 8 * (G & 1), hr = 8 * ((gi / 4) & 1);
+  int kaddr[2][D / 64], vaddr[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = 16 * (gi / 4) + (hr ^ (8 * h)) + gi % 4;  // its swizzle is that of the lane, whatever the tile
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) kaddr[h][u] = row * D + 16 * ((G * (D / 64) + u) ^ C::kswz(row));
+    vaddr[h] = kHalf + gi * 64 + 16 * (G ^ C::vswz(gi)) + (hk ^ (8 * h));
+  }
+
+  f32x4 o[D / 16][2];
+  float m[2], l[2];
+  bool nan_found = false;
+
+  f32x4 s[2][2][2];  // [half][key tile][query tile]
+  vec8 pf[2][2];     // [half][query tile]
+  float sum[2];
+  auto qk = [&](const uint8_t* tile8, int h) {
+    constexpr int kReads = 2 * (D / 64);  // read r: key tile r / (D / 64), chunk r % (D / 64)
+    u32x4 kw[kReads];
+#pragma unroll
+    for (int r = 0; r < kReads; ++r)
+      kw[r] = *reinterpret_cast<const u32x4*>(tile8 + kaddr[h][r % (D / 64)] + 4 * (r / (D / 64)) * D);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) s[h][t][0] = s[h][t][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < kReads; ++r) {
+      const int t = r / (D / 64), u = r % (D / 64);
+      const vec8 k0 = From8<T>::cvt(kw[r][0], kw[r][1]), k1 = From8<T>::cvt(kw[r][2], kw[r][3]);
+      s[h][t][0] = Mfma<T>::mma(k0, qf[0][2 * u], s[h][t][0]);
+      s[h][t][1] = Mfma<T>::mma(k0, qf[1][2 * u], s[h][t][1]);
+      s[h][t][0] = Mfma<T>::mma(k1, qf[0][2 * u + 1], s[h][t][0]);
+      s[h][t][1] = Mfma<T>::mma(k1, qf[1][2 * u + 1], s[h][t][1]);
+    }
+  };
+  auto mask = [&](int j, int h) {
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) {
+      const int left = here(vis[qt] - 64 * j - 16 * G - (hk ^ (8 * h)));
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (x >= left) s[h][x / 4][qt][x % 4] = kNegInf;
+    }
+  };
+  auto row_max = [&](int h, int qt) {
+    float mx = s[h][0][qt][0];
+#pragma unroll
+    for (int x = 1; x < 8; ++x) mx = __builtin_elementwise_maximum(mx, s[h][x / 4][qt][x % 4]);
+    return max_quarters(mx);
+  };
+  auto raise = [&](int h, float c, float ev) {
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) m[qt] = __builtin_elementwise_maximum(m[qt], __builtin_fmaf(row_max(h, qt), c, ev));
+  };
+  auto key_scale = [&](int j) {
+    const float c = a.scale_log2 * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks64), j & 63));
+    return c > 0x1p-126f ? c : 0x1p-126f;  // so that a masked score of -inf times c is -inf
+  };
+  auto exps = [&](int h, float c, float ev) {
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) {
+      const float off = m[qt] == kNegInf ? ev : ev - m[qt];
+      sum[qt] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const float p = fast_exp2(__builtin_fmaf(s[h][x / 4][qt][x % 4], c, off));
+        sum[qt] += p;
+        pf[h][qt][x] = from_f32<T>(p);
+      }
+    }
+  };
+  auto pv = [&](const uint8_t* tile8, int h) {
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(tile8 + vaddr[h] + dt * (16 * 64));
+      const vec8 v = From8<T>::cvt(w[0], w[1]);
+      o[dt][0] = Mfma<T>::mma(v, pf[h][0], o[dt][0]);
+      o[dt][1] = Mfma<T>::mma(v, pf[h][1], o[dt][1]);
+    }
+  };
+  // The same where some row sees the block in part: NaN count as zero here, and are put
+  // where they belong at the end.
+  auto pv_part = [&](const uint8_t* tile8, int h) {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      u32x2 w = *reinterpret_cast<const u32x2*>(tile8 + vaddr[h] + dt * (16 * 64));
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t nan = nan_bytes(w[x]);
+        bad |= nan;
+        w[x] &= ~((nan - (nan >> 7)) | nan);
+      }
+      const vec8 v = From8<T>::cvt(w[0], w[1]);
+      o[dt][0] = Mfma<T>::mma(v, pf[h][0], o[dt][0]);
+      o[dt][1] = Mfma<T>::mma(v, pf[h][1], o[dt][1]);
+    }
+    if (__ballot(bad != 0)) nan_found = true;
+  };
+
+  bool dirty = false, exact = false;
+  auto block = [&](int j, int slot, auto kind) {
+    constexpr bool part = decltype(kind)::value;  // some row of the wave sees the block in part
+    const uint8_t* tile8 = ring + slot * kSlot;
+    const float c = key_scale(j);
+    const int e = exponent_of(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs64), j & 63)));
+    const float ev = (float)e, unit = pow2i(-e);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      qk(tile8, h);
+      if constexpr (part) mask(j, h);
+      if (h == 0 && j == j0 && !exact) raise(h, c, ev);
+      exps(h, c, ev);
+      if (__ballot(!(sum[0] <= kMaxSum<T> && sum[1] <= kMaxSum<T>))) dirty = true;
+      l[0] = __builtin_fmaf(sum[0], unit, l[0]);
+      l[1] = __builtin_fmaf(sum[1], unit, l[1]);
+      if constexpr (part) pv_part(tile8, h);
+      else pv(tile8, h);
+    }
+  };
+  // Blocks before `whole` are seen whole by every row of the wave that sees any token.
+  const int whole = own == 0 ? 0 : least / 64 < j1 ? least / 64 : j1;
+  int j, slot;
+  auto begin = [&] {
+    j = j0, slot = 0;
+    scales(j0 & ~63);
+    fetch(j0, 0);
+    if (j0 + 1 < j1) fetch(j0 + 1, 1);
+  };
+  auto next = [&] {
+    if (j + 1 < j1) wait_vmcnt<2 * kLoads>();
+    else wait_vmcnt<0>();
+    __syncthreads();  // block j has landed, and the one before it is read by all
+    if ((j & 63) == 0 && j > j0) scales(j);
+    if (j + 2 < j1) fetch(j + 2, slot == 0 ? 2 : slot - 1);
+  };
+  m[0] = m[1] = kNegInf;
+  for (;;) {
+    l[0] = l[1] = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int qt = 0; qt < 2; ++qt) o[dt][qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (j0 >= j1) break;
+    begin();
+    for (; j < whole; ++j) {
+      next();
+      block(j, slot, Flag<false>{});
+      slot = slot == 2 ? 0 : slot + 1;
+    }
+    for (; j < j1; ++j) {
+      next();
+      if (64 * j < own) block(j, slot, Flag<true>{});
+      slot = slot == 2 ? 0 : slot + 1;
+    }
+    if (lane == 0) wave_dirty[wave] = dirty ? 1 : 0;
+    __syncthreads();  // the ring is free, the flags are there
+    if (exact || !(wave_dirty[0] | wave_dirty[1] | wave_dirty[2] | wave_dirty[3])) break;  // workgroup-uniform
+    exact = true;
+    begin();
+    for (; j < j1; ++j, slot = slot == 2 ? 0 : slot + 1) {  // the rows' maxima
+      next();
+      if (64 * j >= own) continue;
+      const float c = key_scale(j);
+      const float ev = (float)exponent_of(
+          __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs64), j & 63)));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        qk(ring + slot * kSlot, h);
+        if (j >= whole) mask(j, h);
+        raise(h, c, ev);
+      }
+    }
+    __syncthreads();
+  }
+  if (nan_found) {  // wave-uniform, rare: rows that see a NaN among the values get one
+    for (int j = whole > j0 ? whole : j0; j < j1 && 64 * j < own; ++j) {
+      const uint8_t* vj = vhead + (int64_t)j * kHalf + gi * 64 + 16 * G;
+      vec8 seen[2][2];
+#pragma unroll
+      for (int qt = 0; qt < 2; ++qt)
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          seen[x / 8][qt][x % 8] = from_f32<T>(64 * j + 16 * G + x < vis[qt] ? 1.0f : 0.0f);
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) {
+        u32x4 is = *reinterpret_cast<const u32x4*>(vj + dt * (16 * 64));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) is[x] = nan_bytes(is[x]) >> 7 << 3;  // a positive number for each NaN
+        const vec8 i0 = From8<T>::cvt(is[0], is[1]), i1 = From8<T>::cvt(is[2], is[3]);
+#pragma unroll
+        for (int qt = 0; qt < 2; ++qt) {
+          f32x4 hit = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          hit = Mfma<T>::mma(i0, seen[0][qt], hit);
+          hit = Mfma<T>::mma(i1, seen[1][qt], hit);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (hit[i] > 0.0f) o[dt][qt][i] = __builtin_nanf("");
+        }
+      }
+    }
+  }
+  __syncthreads();  // the ring is free
+
+  if (nblk > p.per) {
+    const int64_t part = part_at(a, p, split, bh, 8 * tile + 2 * wave);
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) {
+      float* po = p.o + (part + qt) * (16 * D) + gi * D + 4 * G;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt) = o[dt][qt];
+      const float all = sum_quarters(l[qt]);
+      if (G == 0) {
+        float* ml = p.ml + (part + qt) * 32 + 2 * gi;
+        ml[0] = vis[qt] > 64 * j0 ? m[qt] : kNegInf;  // a row that saw none of this part
+        ml[1] = vis[qt] > 64 * j0 ? all : 0.0f;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int qt = 0; qt < 2; ++qt) {
+    const float all = sum_quarters(l[qt]);
+    const bool empty = vis[qt] == 0 || all == 0.0f;
+    const float inv = 1.0f / all;
+    const int row = 32 * wave + 16 * qt + gi;
+    uint8_t* orow = ring + row * (2 * D);
+    const int swz = (row / (128 / D)) % (D / 8);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      u32x2 w;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        w[x] = bits16(from_f32<T>(empty ? 0.0f : o[dt][qt][2 * x] * inv)) |
+               (bits16(from_f32<T>(empty ? 0.0f : o[dt][qt][2 * x + 1] * inv)) << 16);
+      *reinterpret_cast<u32x2*>(orow + 16 * ((2 * dt + G / 2) ^ swz) + 8 * (G % 2)) = w;
+    }
+    const int r = kRows * tile + row;
+    if (a.lse && G == 0 && r < rows)
+      a.lse[lse_at(a, b, kvh, r)] = empty ? kNegInf : (m[qt] + __builtin_log2f(all)) * kLn2;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kRows * (D / 8) / 256; ++u) {
+    const int piece = tid + 256 * u, row = piece / (D / 8), c = piece % (D / 8);
+    const int r = kRows * tile + row;
+    if (r >= rows) continue;
+    *reinterpret_cast<u32x4*>(out_row<T>(a, b, kvh, r) + 8 * c) =
+        *reinterpret_cast<const u32x4*>(ring + row * (2 * D) + 16 * (c ^ ((row / (128 / D)) % (D / 8))));
+  }
 }
 
-Few plan_few(const CacheAttn& a) {
-  Few f{};
-  f.tiles = (a.group * a.S + 15) / 16;
-  const int64_t work = (int64_t)a.c.B * a.c.H * f.tiles;
-  const int64_t blocks = (a.max_len + 63) / 64;
-  int64_t splits = (1024 + work - 1) / work;
-  if (splits > blocks / 4) splits = blocks / 4;
-  f.splits = (int)(splits < 1 ? 1 : splits);
-  return f;
+// Tiles of 32 rows straight from memory up to here, of 128 through LDS above.  us, 8 heads
+// over 1000 (9000) tokens, bf16, D = 128: 24 rows 18 (22) against 24 (26), 64 rows 18 (23)
+// against 25 (27), 96 rows 18 (25) against 25 (30), 128 rows 18 (31) against 26 (31).
+constexpr int kFewRows = 96;
+enum Kind { kFew16, kFew32, kMany };
+
+Kind kind_of(const CacheAttn& a) {
+  const int rows = a.group * a.S;
+  return rows <= 16 ? kFew16 : rows <= kFewRows ? kFew32 : kMany;
 }
 
-size_t few_bytes(const CacheAttn& a, const Few& f, int D) {
-  return f.splits > 1 ? (size_t)a.c.B * a.c.H * f.tiles * f.splits * 16 * (D + 2) * sizeof(float) : 0;
+// The walks are split where there are too few to fill the chip and to even out items of
+// different lengths, into parts of at least 8 blocks; a short history is walked at once.
+constexpr int64_t kFewParts = 1024, kFewBlocks = 8, kOnePart = 16;
+constexpr int64_t kManyParts = 2304, kManyBlocks = 8;
+constexpr int64_t kJoinRows = 4096;
+
+Parts plan(const CacheAttn& a) {
+  Parts p{};
+  const Kind kind = kind_of(a);
+  const int64_t rows = (int64_t)a.group * a.S, blocks = ((int64_t)a.max_len + 63) / 64;
+  const int wide = kind == kMany ? 128 : kind == kFew32 ? 32 : 16;
+  const int64_t walks = (int64_t)a.c.B * a.c.H * ((rows + wide - 1) / wide);
+  p.tiles = (int)((rows + wide - 1) / wide * (wide / 16));
+  int64_t per = blocks;
+  if (kind == kMany) {
+    const int64_t splits = (kManyParts + walks - 1) / walks;
+    per = (blocks + splits - 1) / splits;
+    if (per < kManyBlocks) per = kManyBlocks;
+  } else if (blocks > kOnePart) {
+    const int64_t want = (blocks * walks + kFewParts - 1) / kFewParts;
+    per = (want + 3) / 4 * 4;
+    if (per < kFewBlocks) per = kFewBlocks;
+  }
+  p.per = (int)(per < blocks ? per : blocks);
+  p.splits = (int)((blocks + p.per - 1) / p.per);
+  return p;
 }
 
 template <typename T, int D>
 hipError_t launch(const CacheAttn& a, hipStream_t stream) {
-  Few f = plan_few(a);
-  const int64_t parts = (int64_t)a.c.B * a.c.H * f.tiles * f.splits;
-  f.part_o = reinterpret_cast<float*>(a.workspace);
-  f.part_ml = f.part_o + parts * 16 * D;
-  hipLaunchKernelGGL((few_rows_kernel<T, D>), dim3((uint32_t)parts), dim3(256), 0, stream, a, f);
-  if (f.splits > 1)
-    hipLaunchKernelGGL((join_kernel<T, D>), dim3((uint32_t)(parts / f.splits)), dim3(256), 0, stream, a, f);
+  Parts p = plan(a);
+  const Kind kind = kind_of(a);
+  const int64_t heads = (int64_t)a.c.B * a.c.H, total = heads * a.group * a.S;
+  p.o = reinterpret_cast<float*>(a.workspace);
+  p.ml = p.o + heads * p.tiles * p.splits * 16 * D;
+  const int wide = kind == kMany ? 128 : kind == kFew32 ? 32 : 16;
+  const int64_t walks = heads * p.splits, each = p.tiles / (wide / 16);  // few rows: in whole rounds of the XCDs
+  const dim3 grid((uint32_t)((kind == kMany ? walks : (walks + kNumXcd - 1) / kNumXcd * kNumXcd) * each)), threads(256);
+  if (kind == kMany)
+    hipLaunchKernelGGL((many_rows_kernel<T, D>), grid, threads, 0, stream, a, p);
+  else if (kind == kFew32)
+    hipLaunchKernelGGL((few_rows_kernel<T, D, 2>), grid, threads, 0, stream, a, p);
+  else
+    hipLaunchKernelGGL((few_rows_kernel<T, D, 1>), grid, threads, 0, stream, a, p);
+  if (p.splits > 1) {
+    if (total <= kJoinRows)
+      hipLaunchKernelGGL((join_kernel<T, D, 64>), dim3((uint32_t)((total + 3) / 4)), threads, 0, stream, a, p, wide, total);
+    else
+      hipLaunchKernelGGL((join_kernel<T, D, 16>), dim3((uint32_t)((total + 15) / 16)), threads, 0, stream, a, p, wide, total);
+  }
   return hipGetLastError();
 }
 
 }  // namespace
 
-size_t cache_attn_workspace(const CacheAttn& a, int D) { return few_bytes(a, plan_few(a), D); }
+size_t cache_attn_workspace(const CacheAttn& a, int D) {
+  const Parts p = plan(a);
+  return p.splits > 1 ? (size_t)a.c.B * a.c.H * p.tiles * p.splits * 16 * (D + 2) * sizeof(float) : 0;
+}
 
 hipError_t launch_cache_attn(const CacheAttn& a, int dtype, int D, hipStream_t stream) {
   if (dtype == LCV_BSA_F16) return D == 64 ? launch<f16, 64>(a, stream) : launch<f16, 128>(a, stream);

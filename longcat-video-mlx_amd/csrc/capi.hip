@@ -1003,7 +1003,7 @@ int check_cache(const char* name, const lcv_bsa_cache8& c) {
   if (c.capacity % lcv::kCacheBlock)
     return fail(LCV_BSA_ERR_SHAPE, "%s: capacity %lld is not a multiple of %d", name, (long long)c.capacity,
                 lcv::kCacheBlock);
-  if (c.capacity > ((int64_t)1 << 30) || c.B > kI32Max || c.H > kI32Max || c.B * c.H > kI32Max ||
+  if (c.capacity > ((int64_t)1 << 24) || c.B > kI32Max || c.H > kI32Max || c.B * c.H > kI32Max ||
       c.B * c.H * (c.capacity / lcv::kCacheBlock) > kI32Max / 2)
     return fail(LCV_BSA_ERR_UNSUPPORTED, "%s: too many blocks", name);
   if (((uintptr_t)c.k8 | (uintptr_t)c.v8) & 15u)
