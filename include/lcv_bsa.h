@@ -529,14 +529,19 @@ int lcv_bsa_cached_attn(const void* q, int dtype, int64_t Hq, int64_t S,
  * What each cached token got from these queries: out[b,h,j] = weights[b,h,j] +
  * the sum over the queries of key head h that see token j of exp(sm_scale q.k_j -
  * lse), with lse from lcv_bsa_cached_attn.  weights (null: zeros) and out are
- * [B,H,capacity] fp32, and may be one.  The sums' order is fixed.
+ * [B,H,capacity] fp32, and may be one.  The sums' order is fixed.  The workspace
+ * holds the sums of parts of the rows.
  */
+size_t lcv_bsa_attention_weights_workspace_bytes(int64_t Hq, int64_t S,
+                                                 lcv_bsa_cache8 c,
+                                                 int64_t max_len);
 int lcv_bsa_attention_weights(const void* q, int dtype, int64_t Hq, int64_t S,
                               lcv_bsa_strides qs, lcv_bsa_cache8 c,
                               const int32_t* lengths, const int32_t* q_lens,
                               int causal, float sm_scale, int64_t max_len,
                               const float* lse, const float* weights,
-                              float* out, void* stream);
+                              float* out, void* workspace,
+                              size_t workspace_bytes, void* stream);
 
 /*
  * Cuts a cache down: of each head's lengths[b] tokens the newest `recent` stay and

@@ -15,49 +15,13 @@
 // The rows of one key head are its group's queries, row r = query r / group of the
 // group's head r % group; a row sees the first `vis` tokens, rows in order no fewer.  What a row does not see has P' = 0, and
 // a NaN among the values of such tokens is taken out of its product.
-#include "attn_common.h"
-#include "cache_common.h"
+#include "cache_attn.h"
 
 namespace lcv {
 namespace {
 
-// dma16 where the descriptor may have been brought back from spilled lanes right
-// before: a vector instruction's scalar result needs five wait states until a buffer
-// load reads it, and the compiler does not see the load inside the asm.
-__device__ __forceinline__ void dma16_settled(__amdgpu_buffer_rsrc_t rsrc, uint32_t voffset, int32_t soffset,
-                                              uint32_t m0v) {
-  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
-               ::"v"(voffset), "s"(rsrc), "s"(soffset), "{m0}"(m0v)
-               : "memory");
-}
-
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLn2 = 0.69314718055994531f;
-
-struct Lens {
-  int len, ql;  // tokens held, real queries
-};
-__device__ __forceinline__ Lens item_lens(const CacheAttn& a, int b) {
-  Lens r;
-  r.len = a.lengths[b];
-  r.len = r.len < 0 ? 0 : r.len > a.max_len ? a.max_len : r.len;
-  r.ql = a.q_lens ? a.q_lens[b] : a.S;
-  r.ql = r.ql < 0 ? 0 : r.ql > a.S ? a.S : r.ql;
-  return r;
-}
-// Tokens that query i sees.
-__device__ __forceinline__ int visible(const CacheAttn& a, const Lens& n, int i) {
-  if (i >= n.ql) return 0;
-  if (!a.causal) return n.len;
-  const int v = n.len - n.ql + i + 1;
-  return v < 0 ? 0 : v;
-}
-
-// Keeps what follows from being computed before the branch that it stands in.
-__device__ __forceinline__ int here(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
 
 // What the rows [r0, r1) of a key head see: the most of any, and the least of those that
 // see any token.
@@ -390,11 +354,6 @@ struct Tile8 {
   static constexpr int kKeyChunks = D / 16;  // of a key's row
   __device__ static int kswz(int r) { return D == 128 ? ((r >> 4) << 1 | ((r >> 1) & 1)) : r >> 4; }
   __device__ static int vswz(int d) { return (d >> 2) & 3; }
-};
-
-template <bool B>
-struct Flag {
-  static constexpr bool value = B;
 };
 
 template <typename T, int D>

@@ -1050,6 +1050,22 @@ int check_cache_attn(const void* q, int dtype, int64_t Hq, int64_t S, const lcv_
   return LCV_BSA_OK;
 }
 
+// The sizes that a workspace goes by; false where a call of them would be refused.
+bool workspace_shape(int64_t Hq, int64_t S, const lcv_bsa_cache8& c, int64_t max_len, lcv::CacheAttn* a) {
+  if (c.B <= 0 || c.H <= 0 || c.capacity <= 0 || Hq < c.H || S <= 0 || max_len <= 0 || S > kI32Max ||
+      Hq / c.H > kI32Max || (Hq / c.H) * S > kI32Max / 64 || c.B > kI32Max || c.H > kI32Max ||
+      c.capacity > ((int64_t)1 << 24))
+    return false;
+  *a = lcv::CacheAttn{};
+  a->c.B = (int32_t)c.B;
+  a->c.H = (int32_t)c.H;
+  a->c.nb = (int32_t)(c.capacity / lcv::kCacheBlock);
+  a->group = (int32_t)(Hq / c.H);
+  a->S = (int32_t)S;
+  a->max_len = (int32_t)max_len;
+  return true;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1121,15 +1137,8 @@ int lcv_bsa_cache_append(lcv_bsa_cache8 c, const void* k, const void* v, int dty
 }
 
 size_t lcv_bsa_cached_attn_workspace_bytes(int64_t Hq, int64_t S, lcv_bsa_cache8 c, int64_t max_len) {
-  if (c.B <= 0 || c.H <= 0 || Hq < c.H || S <= 0 || max_len <= 0 || Hq * S > kI32Max) return 0;
-  lcv::CacheAttn a{};
-  a.c.B = (int32_t)c.B;
-  a.c.H = (int32_t)c.H;
-  a.c.nb = (int32_t)(c.capacity / lcv::kCacheBlock);
-  a.group = (int32_t)(Hq / c.H);
-  a.S = (int32_t)S;
-  a.max_len = (int32_t)max_len;
-  return lcv::cache_attn_workspace(a, (int)c.D);
+  lcv::CacheAttn a;
+  return workspace_shape(Hq, S, c, max_len, &a) ? lcv::cache_attn_workspace(a, (int)c.D) : 0;
 }
 
 int lcv_bsa_cached_attn(const void* q, int dtype, int64_t Hq, int64_t S, lcv_bsa_strides qs, lcv_bsa_cache8 c,
@@ -1150,14 +1159,26 @@ int lcv_bsa_cached_attn(const void* q, int dtype, int64_t Hq, int64_t S, lcv_bsa
   return launch_status(lcv::launch_cache_attn(a, dtype, (int)c.D, (hipStream_t)stream), "lcv_bsa_cached_attn");
 }
 
+size_t lcv_bsa_attention_weights_workspace_bytes(int64_t Hq, int64_t S, lcv_bsa_cache8 c, int64_t max_len) {
+  lcv::CacheAttn a;
+  return workspace_shape(Hq, S, c, max_len, &a) ? lcv::cache_weights_workspace(a, (int)c.D) : 0;
+}
+
 int lcv_bsa_attention_weights(const void* q, int dtype, int64_t Hq, int64_t S, lcv_bsa_strides qs, lcv_bsa_cache8 c,
                               const int32_t* lengths, const int32_t* q_lens, int causal, float sm_scale,
-                              int64_t max_len, const float* lse, const float* weights, float* out, void* stream) {
+                              int64_t max_len, const float* lse, const float* weights, float* out, void* workspace,
+                              size_t workspace_bytes, void* stream) {
   lcv::CacheAttn a;
   const int st = check_cache_attn(q, dtype, Hq, S, qs, c, lengths, q_lens, causal, sm_scale, max_len, &a);
   if (st) return st;
   if (!lse || !out) return fail(LCV_BSA_ERR_INVALID_ARG, "null pointer");
+  if (qs.s >= (int64_t)1 << 25)  // 32 rows are addressed in 32 bits
+    return fail(LCV_BSA_ERR_LAYOUT, "q's rows are 2^25 elements or more apart");
   a.lse = const_cast<float*>(lse);
+  const size_t need = lcv::cache_weights_workspace(a, (int)c.D);
+  if (workspace_bytes < need || (need && (!workspace || (uintptr_t)workspace % 16)))
+    return fail(LCV_BSA_ERR_INVALID_ARG, "workspace of %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
+  a.workspace = workspace;
   return launch_status(lcv::launch_cache_weights(a, dtype, (int)c.D, weights, out, (hipStream_t)stream),
                        "lcv_bsa_attention_weights");
 }

@@ -119,7 +119,9 @@ _SIGNATURES = {
     "lcv_bsa_cached_attn": (c_int, [c_void_p, c_int, c_int64, c_int64, Strides, Cache8, c_void_p, c_void_p, c_int,
                                     c_float, c_int64, c_void_p, Strides, c_void_p, c_void_p, c_size_t, c_void_p]),
     "lcv_bsa_attention_weights": (c_int, [c_void_p, c_int, c_int64, c_int64, Strides, Cache8, c_void_p, c_void_p, c_int,
-                                          c_float, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+                                          c_float, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                          c_void_p]),
+    "lcv_bsa_attention_weights_workspace_bytes": (c_size_t, [c_int64, c_int64, Cache8, c_int64]),
     "lcv_bsa_cache_evict": (c_int, [Cache8, c_void_p, c_void_p, c_int64, c_int64, Cache8, c_void_p, c_void_p, c_void_p,
                                     c_void_p]),
 }

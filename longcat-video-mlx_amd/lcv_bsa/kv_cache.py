@@ -263,14 +263,20 @@ def attention_weights(q: torch.Tensor, cache: KVCache8, lengths: Ints, lse: torc
         raise ValueError("out must be contiguous")
     if q.numel() == 0 or max_len == 0:
         return out.zero_() if weights is None else out.copy_(weights) if out is not weights else out
+    if q.stride(2) >= 1 << 25:  # beyond what the kernel's row offsets hold
+        q = q.contiguous()
     q, qs = rows_of(q, "q")
     lse = lse.contiguous()
     weights = None if weights is None else weights.contiguous()
+    lib = _lib.load()
+    size = lib.lcv_bsa_attention_weights_workspace_bytes(Hq, S, cache._c, max_len)
+    ws = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
     with on_device(q):
-        st = _lib.load().lcv_bsa_attention_weights(
+        st = lib.lcv_bsa_attention_weights(
             q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._c, lengths.data_ptr(),
             None if q_lens is None else q_lens.data_ptr(), int(causal), sm_scale, max_len, lse.data_ptr(),
-            None if weights is None else weights.data_ptr(), out.data_ptr(), _stream(q))
+            None if weights is None else weights.data_ptr(), out.data_ptr(), None if ws is None else ws.data_ptr(), size,
+            _stream(q))
     _lib.check(st, "attention_weights")
     return out
 

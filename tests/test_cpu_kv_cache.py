@@ -171,7 +171,7 @@ def test_c_entries_refuse_before_a_launch():
     for c, status in bad:
         assert lib.lcv_bsa_cache_append(c, fake, fake, 1, 4, st, st, fake, None, None) == status
         assert lib.lcv_bsa_cached_attn(fake, 1, 2, 4, st, c, fake, None, 0, 0.1, 64, fake, st, None, None, 0, None) == status
-        assert lib.lcv_bsa_attention_weights(fake, 1, 2, 4, st, c, fake, None, 0, 0.1, 64, fake, None, fake, None) == status
+        assert lib.lcv_bsa_attention_weights(fake, 1, 2, 4, st, c, fake, None, 0, 0.1, 64, fake, None, fake, None, 0, None) == status
         assert lib.lcv_bsa_cache_evict(c, fake, fake, 4, 0, C(), fake, fake, fake, None) == status
         assert lib.lcv_bsa_cache_evict(C(), fake, fake, 4, 0, c, fake, fake, fake, None) == status
 
