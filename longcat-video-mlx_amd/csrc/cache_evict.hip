@@ -1,179 +1,302 @@
 // Eviction from the 8-bit cache (cache_common.h): of each head, the newest `recent`
 // tokens and the heaviest of the others stay, keep in all, in their order.
 //
-// Two kernels.  The first ranks: a radix search over the weights' bits (as unsigned
-// numbers in the order of the floats, NaN below everything) for the weight of the
-// last token to stay, among equals the lowest tokens, then the list of kept tokens in
-// order.  The second gathers: one workgroup makes one block of the new cache, whose
-// scale is the least one for the rows it gets.
+// Two kernels.  The first ranks, one workgroup a head: weights as unsigned numbers in the
+// order of the floats (NaN below everything), held in LDS, and a search for the number T
+// of the last token to stay (count above T < want <= count from T on).  A round sorts the
+// candidates into 4096 bins of the interval [a, z) by a shift, and goes on in the bin where
+// the count passes `want`: three rounds at most, whatever the weights.  As soon as 512 are
+// left they are compared with one another.  Each wave holds a run of tokens, so one
+// exchange of the waves' counts places every kept token; equal weights at T stay from the
+// lowest token on.
+//
+// The second gathers: one workgroup makes one block of the new cache, whose scale is the
+// least one for the rows it gets.  Keys move as 32-byte pieces of rows; of the values,
+// whose bytes lie token by token, a wave takes one of the D rows at a time, its lanes the
+// 64 tokens: kept tokens are in order, so the lanes' bytes are in few lines.
 #include "cache_common.h"
 
 namespace lcv {
 namespace {
 
-// Floats as unsigned numbers of the same order; -0 as +0, NaN last.
+// Floats as unsigned numbers of the same order, from 1; -0 as +0, NaN first.
 __device__ __forceinline__ uint32_t rank_bits(float w) {
-  if (w != w) return 0u;
+  if (w != w) return 1u;
   const uint32_t u = __builtin_bit_cast(uint32_t, w == 0.0f ? 0.0f : w);
   return (u >> 31) ? ~u : u | 0x80000000u;
 }
+constexpr uint32_t kAlways = ~0u;          // the newest tokens' key; 0: no token
+constexpr uint64_t kKeysEnd = 0xff800001;  // past infinity's
 
-constexpr int kRankThreads = 1024;
+constexpr int kRankThreads = 1024, kRankWaves = kRankThreads / 64;
+constexpr int kBins = 4096;
+constexpr uint32_t kLast = 512;
 
-__global__ __launch_bounds__(kRankThreads) void rank_kernel(const int32_t* lengths, const float* weights, int H,
-                                                            int64_t capacity, int keep, int recent,
-                                                            int64_t new_capacity, int32_t* kept, float* w_out,
-                                                            int32_t* new_lengths) {
-  __shared__ uint32_t hist[256];
+// N: keys that LDS holds, or 0 where the weights are read anew at each pass.  (In
+// registers the loops over them would be unrolled, and a launch that runs each
+// instruction a few times waits for the instructions: 38 us for 18,720 tokens.)
+template <int N>
+__global__ __launch_bounds__(kRankThreads) void rank_kernel(const int32_t* lengths, const float* __restrict__ weights,
+                                                            int H, int64_t capacity, int keep, int recent,
+                                                            int32_t* __restrict__ kept, int32_t* new_lengths) {
+  __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];  // later: the last candidates
+  __shared__ uint32_t waves[2][kRankWaves];
   __shared__ uint32_t found[3];
-  __shared__ uint32_t wave_ties[16], wave_kept[16];
+  __shared__ uint32_t held[N + 192];  // past the end: read four at a time
   const int bh = blockIdx.x, b = bh / H;
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-  int64_t len = lengths[b];
-  len = len < 0 ? 0 : len > capacity ? capacity : len;
-  const int64_t tail = recent < len ? recent : len;
-  const int64_t old = len - tail;  // tokens that compete
-  const int64_t left = len < keep ? len : keep;
-  int64_t want = left - tail;  // of them stay
+  const int tid = threadIdx.x, lane = tid % 64, wave = uniform_i32(tid / 64);
+  int64_t n = lengths[b];
+  const int len = (int)(n < 0 ? 0 : n > capacity ? capacity : n);
+  const int tail = recent < len ? recent : len;
+  const int old = len - tail;  // tokens that compete
+  const int left = len < keep ? len : keep;
+  const int want = left - tail;  // of them stay
   const float* w = weights + (int64_t)bh * capacity;
 
-  // The search: after each pass `prefix` holds the top bits of the last kept weight
-  // and `want` its place among the weights that share them.
-  uint32_t prefix = 0, mask = 0;
-  const bool all = want >= old;
-  if (!all && want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int64_t i = tid; i < old; i += kRankThreads) {
-        const uint32_t u = rank_bits(w[i]);
-        if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255u], 1u);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        uint32_t above = 0;
-        int d = 255;
-        for (; d > 0 && above + hist[d] < (uint32_t)want; --d) above += hist[d];
-        found[0] = (uint32_t)d;
-        found[1] = above;
-      }
-      __syncthreads();
-      prefix |= found[0] << shift;
-      mask |= 255u << shift;
-      want -= found[1];
-      __syncthreads();
+  // Wave w holds tokens w * run .. + run - 1, its lane l tokens r * 64 + l of them.
+  const int per = (len + kRankThreads - 1) / kRankThreads, run = per * 64, first = wave * run + lane;
+  // Some weights at a time, so that their loads (from memory or LDS) are under way together;
+  // the compiler unrolls no loop over ballots.
+  auto keys = [&](int r0, auto& k) {
+    constexpr int n = sizeof(k) / 4;
+    float x[n];
+#pragma unroll
+    for (int q = 0; q < n; ++q) {
+      const int i = first + 64 * (r0 + q);
+      x[q] = w[i < old ? i : 0];  // capacity > 0
+    }
+#pragma unroll
+    for (int q = 0; q < n; ++q) {
+      const int i = first + 64 * (r0 + q);
+      k[q] = r0 + q >= per ? 0u : i < old ? rank_bits(x[q]) : i < len ? kAlways : 0u;
+    }
+  };
+  if constexpr (N > 0) {
+    for (int r = 0; r < per; r += 8) {
+      uint32_t k[8];
+      keys(r, k);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (r + q < per) held[first + 64 * (r + q)] = k[q];  // read by the same lane alone
     }
   }
-  // The list, in order: a token stays if it is newest, above the threshold, or one of
-  // the first `want` at it.
-  uint32_t ties = 0, out = 0;
-  for (int64_t i0 = 0; i0 < len; i0 += kRankThreads) {
-    const int64_t i = i0 + tid;
-    const float wi = i < len ? w[i] : 0.0f;
-    const uint32_t u = rank_bits(wi);
-    const bool race = i < old && !all && left > tail;
-    const bool tie = race && u == prefix;
-    const uint64_t tie_mask = __ballot(tie);
-    if (lane == 0) wave_ties[wave] = (uint32_t)__popcll(tie_mask);
-    __syncthreads();
-    uint32_t before = ties, tie_total = 0;
-    for (int k = 0; k < 16; ++k) {
-      if (k < wave) before += wave_ties[k];
-      tie_total += wave_ties[k];
+  // f(i, key) for every token of this lane; key 0 behind the last.
+  auto each = [&](auto f) {
+    for (int r = 0; r < per; r += 4) {
+      uint32_t k[4];
+      if constexpr (N > 0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) k[q] = held[first + 64 * (r + q)];
+#pragma unroll
+        for (int q = 1; q < 4; ++q) k[q] = r + q < per ? k[q] : 0u;
+      } else {
+        keys(r, k);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f(first + 64 * (r + q), k[q]);
     }
-    before += mbcnt64(tie_mask);
-    const bool stay = i < len && (i >= old || (i < old && all) || (race && u > prefix) || (tie && before < (uint32_t)want));
-    const uint64_t stay_mask = __ballot(stay);
-    if (lane == 0) wave_kept[wave] = (uint32_t)__popcll(stay_mask);
-    __syncthreads();
-    uint32_t at = out, total = 0;
-    for (int k = 0; k < 16; ++k) {
-      if (k < wave) at += wave_kept[k];
-      total += wave_kept[k];
+  };
+
+  // T: the largest key that at least `want` competing tokens reach; the first `ties` of
+  // those equal to T stay beside all that exceed it.
+  uint32_t T = want >= old ? 0u : kAlways - 1, ties = 0;
+  if (want < old && want > 0) {
+    const uint32_t goal = (uint32_t)want;
+    uint64_t a = 1, z = kKeysEnd;
+    uint32_t above = 0, have = (uint32_t)old;  // keys from z on; keys in [a, z)
+    while (z - a > 1 && have > kLast) {        // workgroup-uniform
+      int shift = 0;
+      while ((z - a - 1) >> shift >= kBins) ++shift;
+      reinterpret_cast<u32x4*>(bins)[tid] = u32x4{0u, 0u, 0u, 0u};
+      __syncthreads();
+      each([&](int, uint32_t k) {
+        if (k >= a && k < z) atomicAdd(&bins[(k - (uint32_t)a) >> shift], 1u);
+      });
+      __syncthreads();
+      // Thread t: bins 4 t .. 4 t + 3, and how many keys lie in the bins behind them.
+      const u32x4 c = reinterpret_cast<u32x4*>(bins)[tid];
+      const uint32_t mine = c[0] + c[1] + c[2] + c[3];
+      uint32_t from = mine;
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = __shfl_down(from, o);
+        from += lane + o < 64 ? x : 0u;
+      }
+      if (lane == 0) waves[0][wave] = from;
+      __syncthreads();
+      uint32_t behind = above + from - mine;
+      for (int k = wave + 1; k < kRankWaves; ++k) behind += waves[0][k];
+#pragma unroll
+      for (int q = 3; q >= 0; --q) {
+        if (behind < goal && behind + c[q] >= goal) found[0] = 4 * tid + q, found[1] = behind, found[2] = c[q];
+        behind += c[q];
+      }
+      __syncthreads();
+      a += (uint64_t)found[0] << shift;
+      z = a + ((uint64_t)1 << shift) < z ? a + ((uint64_t)1 << shift) : z;
+      above = found[1], have = found[2];
     }
-    at += mbcnt64(stay_mask);
-    if (stay) {
-      kept[(int64_t)bh * keep + at] = (int32_t)i;
-      w_out[(int64_t)bh * new_capacity + at] = wi;
+    T = (uint32_t)a, ties = goal - above;
+    if (z - a > 1) {  // at most kLast candidates, against one another
+      __syncthreads();
+      if (tid < (int)kLast) bins[tid] = 0;
+      if (tid == 0) found[0] = 0;
+      __syncthreads();
+      each([&](int, uint32_t k) {
+        if (k >= a && k < z) bins[atomicAdd(&found[0], 1u)] = k;  // in any order
+      });
+      __syncthreads();
+      if (tid < (int)have) {
+        const uint32_t k = bins[tid];
+        uint32_t more = above, from = above;
+#pragma unroll 4
+        for (uint32_t i = 0; i < kLast; i += 4) {  // zeros behind the last: none reaches a key
+          const u32x4 x = *reinterpret_cast<const u32x4*>(&bins[i]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            more += x[q] > k ? 1u : 0u;
+            from += x[q] >= k ? 1u : 0u;
+          }
+        }
+        if (more < goal && from >= goal) {  // equal keys write the same
+          found[1] = from == goal ? k - 1 : k;
+          found[2] = from == goal ? 0u : goal - more;
+        }
+      }
+      __syncthreads();
+      T = found[1], ties = found[2];
     }
-    ties += tie_total;
-    out += total;
-    __syncthreads();
   }
-  for (int64_t i = left + tid; i < keep; i += kRankThreads) kept[(int64_t)bh * keep + i] = -1;
-  for (int64_t i = left + tid; i < new_capacity; i += kRankThreads) w_out[(int64_t)bh * new_capacity + i] = 0.0f;
-  if (tid == 0 && bh % H == 0) new_lengths[b] = (int32_t)left;
+  // Where this wave's tokens go, and which ties are its own.
+  uint32_t n_new = 0, n_tie = 0;
+  each([&](int, uint32_t k) {
+    n_new += k > T ? 1u : 0u;
+    n_tie += k == T ? 1u : 0u;  // counted only where there are ties
+  });
+  for (int o = 1; o < 64; o <<= 1) n_new += __shfl_xor(n_new, o), n_tie += __shfl_xor(n_tie, o);
+  __syncthreads();  // waves is read
+  if (lane == 0) waves[0][wave] = n_new, waves[1][wave] = n_tie;
+  __syncthreads();
+  uint32_t at = 0, tie = 0;
+  for (int k = 0; k < wave; ++k) {
+    const uint32_t room = ties - tie, use = waves[1][k] < room ? waves[1][k] : room;
+    at += waves[0][k] + use;
+    tie += use;
+  }
+  int32_t* list = kept + (int64_t)bh * keep;
+  if (ties == 0) {
+    each([&](int i, uint32_t k) {
+      const uint64_t mask = __ballot(k > T);
+      if (k > T) list[at + mbcnt64(mask)] = i;
+      at += (uint32_t)__popcll(mask);
+    });
+  } else {
+    each([&](int i, uint32_t k) {
+      const uint64_t tie_mask = __ballot(k == T);
+      const bool stay = k > T || (k == T && tie + mbcnt64(tie_mask) < ties);
+      const uint64_t mask = __ballot(stay);
+      if (stay) list[at + mbcnt64(mask)] = i;
+      at += (uint32_t)__popcll(mask);
+      tie += (uint32_t)__popcll(tie_mask);
+      tie = tie < ties ? tie : ties;
+    });
+  }
+  for (int i = left + tid; i < keep; i += kRankThreads) list[i] = -1;
+  if (tid == 0 && bh % H == 0) new_lengths[b] = left;
 }
 
-template <int D>
-__global__ __launch_bounds__(256) void gather_kernel(Cache8 src, Cache8 dst, const int32_t* kept, int keep) {
-  __shared__ float wave_max[4];
-  __shared__ __attribute__((aligned(16))) uint8_t tile[64 * (D + 4)];
-  int64_t id = blockIdx.x;
-  const int isv = (int)(id & 1);
-  id >>= 1;
-  const int j = (int)(id % dst.nb);
-  const int64_t bh = id / dst.nb;
-  const int tid = threadIdx.x, row = tid / 4, quarter = tid % 4;
-  const int64_t slot = 64 * (int64_t)j + row;
-  const int64_t cap = (int64_t)src.nb * 64;
-  int64_t t = slot < keep ? kept[bh * keep + slot] : -1;
-  if (t >= cap) t = -1;
-  float x[D / 4];
+// The scale's exponent for what `word` holds under `scale`, over the workgroup, and the
+// words under it.
+template <int W>
+__device__ __forceinline__ float largest(const uint32_t (&word)[W], float scale) {
   float amax = 0.0f;
-  if (t >= 0) {
-    const int64_t block = bh * src.nb + t / 64;
-    const float scale = pow2i(exponent_of((isv ? src.v_scale : src.k_scale)[block]));
-    if (!isv) {
-      const uint8_t* in = src.k8 + block * (64 * D) + (t % 64) * D + quarter * (D / 4);
 #pragma unroll
-      for (int u = 0; u < D / 16; ++u) unpack_e4m3(reinterpret_cast<const uint32_t*>(in)[u], x + 4 * u);
-    } else {
-      const uint8_t* in = src.v8 + block * (64 * D) + (t % 64) + quarter * (D / 4) * 64;
+  for (int i = 0; i < W; ++i) {
+    float y[4];
+    unpack_e4m3(word[i], y);
 #pragma unroll
-      for (int u = 0; u < D / 16; ++u) {
-        uint32_t word = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) word |= (uint32_t)in[(4 * u + e) * 64] << (8 * e);
-        unpack_e4m3(word, x + 4 * u);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) {
-      x[i] *= scale;
-      const float a = __builtin_fabsf(x[i]);
-      amax = a < __builtin_inff() ? fmaxf(amax, a) : amax;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+    for (int e = 0; e < 4; ++e) amax = fmaxf(amax, __builtin_fabsf(y[e]));  // fmaxf leaves NaN out
   }
+  amax *= scale;
   for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-  if (tid % 64 == 0) wave_max[tid / 64] = amax;
-  const bool filled = __syncthreads_or(t >= 0) != 0;
-  amax = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
-  const int e = filled ? scale_exponent(amax) : 0;
-  const float inv = pow2i(-e);
+  return amax;
+}
+template <int W>
+__device__ __forceinline__ void rescale(uint32_t (&word)[W], float by) {
 #pragma unroll
-  for (int u = 0; u < D / 16; ++u)
-    *reinterpret_cast<uint32_t*>(tile + row * (D + 4) + quarter * (D / 4) + 4 * u) =
-        pack_e4m3(x[4 * u] * inv, x[4 * u + 1] * inv, x[4 * u + 2] * inv, x[4 * u + 3] * inv);
-  __syncthreads();
-  const int64_t block = bh * dst.nb + j;
-  if (tid == 0) (isv ? dst.v_scale : dst.k_scale)[block] = pow2i(e);
-  uint8_t* out = (isv ? dst.v8 : dst.k8) + block * (64 * D);
-  for (int i = tid; i < 64 * D / 4; i += 256) {
-    uint32_t word;
-    if (!isv) {
-      word = *reinterpret_cast<const uint32_t*>(tile + i / (D / 4) * (D + 4) + i % (D / 4) * 4);
-    } else {
-      const int d = i / 16, r = i % 16 * 4;
-      word = 0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) word |= (uint32_t)tile[(r + q) * (D + 4) + d] << (8 * q);
-    }
-    reinterpret_cast<uint32_t*>(out)[i] = word;
+  for (int i = 0; i < W; ++i) {
+    float y[4];
+    unpack_e4m3(word[i], y);
+    word[i] = pack_e4m3(y[0] * by, y[1] * by, y[2] * by, y[3] * by);
   }
+}
+
+// One workgroup a block of the new cache, its keys and its values: thread (row, quarter of
+// D) of the keys, (quarter of D, row) of the values.
+template <int D>
+__global__ __launch_bounds__(256) void gather_kernel(Cache8 src, Cache8 dst, const int32_t* __restrict__ kept, int keep,
+                                                     const float* __restrict__ weights, float* __restrict__ w_out) {
+  constexpr int W = D / 16;  // words of a quarter
+  __shared__ float maxima[2][4];
+  const int j = (int)(blockIdx.x % dst.nb);
+  const int64_t bh = blockIdx.x / dst.nb;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const int krow = tid / 4, kd = tid % 4 * (D / 4), vd = wave * (D / 4);
+  const int64_t slot0 = 64 * (int64_t)j, old = bh * src.nb, block = bh * dst.nb + j;
+  auto token = [&](int row) {
+    const int64_t t = slot0 + row < keep ? kept[bh * keep + slot0 + row] : -1;
+    return t < (int64_t)src.nb * 64 ? t : -1;
+  };
+  const int64_t kt = token(krow), vt = token(lane);
+  const bool filled = token(0) >= 0;
+  uint32_t kw[W], vw[W];
+  float ks = 1.0f, vs = 1.0f, weight = 0.0f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) kw[i] = vw[i] = 0;
+  if (kt >= 0) {
+    const u32x4* in = reinterpret_cast<const u32x4*>(src.k8 + (old + kt / 64) * (64 * D) + (kt % 64) * D + kd);
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) kw[4 * i + e] = in[i][e];
+    ks = src.k_scale[old + kt / 64];
+  }
+  if (vt >= 0) {
+    const uint8_t* in = src.v8 + (old + vt / 64) * (64 * D) + vd * 64 + vt % 64;
+    uint8_t byte[4 * W];
+#pragma unroll
+    for (int i = 0; i < 4 * W; ++i) byte[i] = in[i * 64];
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      vw[i] = byte[4 * i] | (uint32_t)byte[4 * i + 1] << 8 | (uint32_t)byte[4 * i + 2] << 16 | (uint32_t)byte[4 * i + 3] << 24;
+    vs = src.v_scale[old + vt / 64];
+    if (wave == 0) weight = weights[old * 64 + vt];
+  }
+  if (wave == 0) w_out[block * 64 + lane] = weight;
+  ks = pow2i(exponent_of(ks));
+  vs = pow2i(exponent_of(vs));
+  const float kmax = largest(kw, ks), vmax = largest(vw, vs);
+  if (lane == 0) maxima[0][wave] = kmax, maxima[1][wave] = vmax;
+  __syncthreads();
+  int e[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    e[i] = filled ? scale_exponent(fmaxf(fmaxf(maxima[i][0], maxima[i][1]), fmaxf(maxima[i][2], maxima[i][3]))) : 0;
+  if (tid == 0) dst.k_scale[block] = pow2i(e[0]), dst.v_scale[block] = pow2i(e[1]);
+  rescale(kw, ks * pow2i(-e[0]));  // by 2^(old - new), within 2^-120 .. 2^120
+  u32x4* out = reinterpret_cast<u32x4*>(dst.k8 + block * (64 * D) + krow * D + kd);
+#pragma unroll
+  for (int i = 0; i < W / 4; ++i) out[i] = u32x4{kw[4 * i], kw[4 * i + 1], kw[4 * i + 2], kw[4 * i + 3]};
+  rescale(vw, vs * pow2i(-e[1]));
+  uint8_t* vout = dst.v8 + block * (64 * D) + vd * 64 + lane;
+#pragma unroll
+  for (int i = 0; i < 4 * W; ++i) vout[i * 64] = (uint8_t)(vw[i / 4] >> (8 * (i % 4)));
+}
+
+template <int N>
+void launch_rank(const Cache8& src, const int32_t* lengths, const float* weights, int keep, int recent,
+                 int32_t* kept, int32_t* new_lengths, hipStream_t stream) {
+  hipLaunchKernelGGL((rank_kernel<N>), dim3(src.B * src.H), dim3(kRankThreads), 0, stream, lengths, weights, src.H,
+                     (int64_t)src.nb * 64, keep, recent, kept, new_lengths);
 }
 
 }  // namespace
@@ -181,13 +304,15 @@ __global__ __launch_bounds__(256) void gather_kernel(Cache8 src, Cache8 dst, con
 hipError_t launch_cache_evict(const Cache8& src, const int32_t* lengths, const float* weights, int keep, int recent,
                               const Cache8& dst, float* w_out, int32_t* kept, int32_t* new_lengths, int D,
                               hipStream_t stream) {
-  hipLaunchKernelGGL(rank_kernel, dim3(src.B * src.H), dim3(kRankThreads), 0, stream, lengths, weights, src.H,
-                     (int64_t)src.nb * 64, keep, recent, (int64_t)dst.nb * 64, kept, w_out, new_lengths);
-  const uint32_t grid = (uint32_t)((int64_t)src.B * src.H * dst.nb * 2);
+  const int64_t most = ((int64_t)src.nb * 64 + kRankThreads - 1) / kRankThreads * kRankThreads;
+  const auto rank = most <= 4096 ? launch_rank<4096> : most <= 16384 ? launch_rank<16384> : most <= 35840 ? launch_rank<35840>
+                                                                                                        : launch_rank<0>;
+  rank(src, lengths, weights, keep, recent, kept, new_lengths, stream);
+  const uint32_t grid = (uint32_t)((int64_t)src.B * src.H * dst.nb);
   if (D == 64)
-    hipLaunchKernelGGL((gather_kernel<64>), dim3(grid), dim3(256), 0, stream, src, dst, kept, keep);
+    hipLaunchKernelGGL((gather_kernel<64>), dim3(grid), dim3(256), 0, stream, src, dst, kept, keep, weights, w_out);
   else
-    hipLaunchKernelGGL((gather_kernel<128>), dim3(grid), dim3(256), 0, stream, src, dst, kept, keep);
+    hipLaunchKernelGGL((gather_kernel<128>), dim3(grid), dim3(256), 0, stream, src, dst, kept, keep, weights, w_out);
   return hipGetLastError();
 }
 

@@ -327,6 +327,13 @@ def test_attention_layouts_and_bounds(device, S):
     (1, 2, 64, 256, [256], 100, 0, "special"),
     (2, 1, 64, 4224, [4200, 1030], 1, 0, "random"),
     (1, 1, 64, 4224, [4220], 4219, 1, "random"),
+    (1, 1, 64, 4224, [4200], 2000, 5, "ties"),
+    (1, 1, 64, 20544, [20500], 9000, 100, "ties"),
+    (1, 1, 64, 20544, [20500], 300, 0, "spread"),
+    (1, 1, 64, 66048, [66000], 100, 3, "ties"),
+    (1, 1, 64, 66048, [65999], 30000, 0, "spread"),
+    (1, 2, 64, 2560, [2500], 1200, 0, "two values"),
+    (1, 1, 64, 2560, [2500], 2400, 0, "special"),
 ])
 def test_evict(device, B, H, D, capacity, lengths, keep, recent, kind):
     from lcv_bsa import cache_evict
@@ -338,6 +345,10 @@ def test_evict(device, B, H, D, capacity, lengths, keep, recent, kind):
         w = (w * 4).floor()
     elif kind == "all equal":
         w.fill_(0.25)
+    elif kind == "two values":
+        w = torch.where(w > 0.5, 1e-38, 3e38)
+    elif kind == "spread":  # every exponent, both signs
+        w = torch.randint(0, 1 << 32, w.shape, generator=gen, device=device, dtype=torch.int64).to(torch.int32).view(torch.float32)
     elif kind == "special":
         w = w * 2 - 1
         w[..., ::7], w[..., 1::9], w[..., 2::11], w[..., 3::13], w[..., 4::5] = math.nan, math.inf, -math.inf, -0.0, 0.0
