@@ -1086,7 +1086,7 @@ int lcv_bsa_rope_nd(const void* x, int dtype, int64_t B, int64_t H, int64_t S, i
   if (axes > D / 2 || !(base > 0.0) || !std::isfinite(base))
     return fail(LCV_BSA_ERR_INVALID_ARG, "at most D / 2 axes and a positive base");
   if (pos_stride_b < 0 || pos_stride_s < 0) return fail(LCV_BSA_ERR_LAYOUT, "position strides must be non-negative");
-  if (B > kI32Max || H > kI32Max || S > kI32Max || B * H > kI32Max || B * S > ((int64_t)1 << 33) || B * H * S > ((int64_t)1 << 40))
+  if (B > kI32Max || H > (1 << 20) || S > kI32Max / 16 || B * S > kI32Max / 2 || B * H * S > ((int64_t)1 << 40))
     return fail(LCV_BSA_ERR_UNSUPPORTED, "tensor too large");
   int st;
   if ((st = check_strides("x", xs, D)) || (st = check_strides("out", os, D))) return st;
