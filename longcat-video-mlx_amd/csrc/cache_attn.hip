@@ -74,20 +74,43 @@ __device__ __forceinline__ int64_t lse_at(const CacheAttn& a, int b, int kvh, in
 // that a lane reads of v8's row 16 dt + gi.  Keys and values of a wave's next block are
 // asked for as soon as those of this one are used.
 template <typename T, int D, int NT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, NT == 1 ? 3 : 2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 1 ? 3 : 2, NT == 1 ? 3 : 2)))
 void few_rows_kernel(CacheAttn a, Parts p) {
   typedef typename Mfma<T>::vec8 vec8;
   __shared__ float part_o[4][16 * D];
   __shared__ float part_ml[4][32];
-  // Work: (part, key head) u, whose tiles follow one another on one XCD (u % 8); heads
-  // next to one another, so that every XCD has some of every item's.
-  const int heads = a.c.B * a.c.H, slot = blockIdx.x / kNumXcd, wide = p.tiles / NT;
+  // Work: (part, key head) u, whose tiles follow one another on one XCD (u % 8), the heads
+  // next to one another.  Only the parts that an item has are counted: a long item beside
+  // short ones then finds the chip free of workgroups that have nothing to do (22 us
+  // against 16 for lengths of 8200, 4097, 1 and 12000).
+  const int slot = blockIdx.x / kNumXcd, wide = p.tiles / NT;
   const int tile = slot % wide * NT;
   const int u = slot / wide * kNumXcd + blockIdx.x % kNumXcd;
-  const int bh = u % heads, split = u / heads;
-  if (split >= p.splits) return;
-  const int b = bh / a.c.H, kvh = bh - b * a.c.H;
   const int lane = threadIdx.x % 64, G = lane / 16, gi = lane % 16;
+  const int kvh = u % a.c.H;
+  int b = a.c.B == 1 ? 0 : -1, split = u / a.c.H;
+  for (int b0 = 0; b < 0 && b0 < a.c.B; b0 += 64) {  // wave-uniform
+    int parts = 0;
+    if (b0 + lane < a.c.B) {
+      const int len = item_lens(a, b0 + lane).len;
+      parts = len > 0 ? ((len + 63) / 64 + p.per - 1) / p.per : 1;
+    }
+    int upto = parts;
+    for (int o = 1; o < 64 && o < a.c.B; o <<= 1) {
+      const int x = __shfl_up(upto, o);
+      upto += lane >= o ? x : 0;
+    }
+    const uint64_t beyond = __ballot(split < upto);
+    if (beyond) {
+      const int l = __builtin_ctzll(beyond);
+      b = b0 + l;
+      split -= __builtin_amdgcn_readlane(upto - parts, l);
+    } else {
+      split -= __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+  if (b < 0) return;
+  const int bh = b * a.c.H + kvh;
   const int wave = uniform_i32(threadIdx.x / 64);
   const Lens n = item_lens(a, b);
   const int rows = a.group * a.S;

@@ -19,6 +19,7 @@ the cache.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Union
 
@@ -50,20 +51,24 @@ class KVCache8:
         if k8.dim() != 4:
             raise ValueError(f"k8 must be [B, H, capacity, D], got shape {tuple(k8.shape)}")
         B, H, n, D = k8.shape
-        if D not in (64, 128) or n < BLOCK or n % BLOCK or B < 1 or H < 1:
+        nb = n // BLOCK
+        if (D != 64 and D != 128) or n < BLOCK or n % BLOCK or B < 1 or H < 1:
             raise ValueError(f"an 8-bit cache holds head dims 64 and 128 and a multiple of {BLOCK} tokens, "
                              f"got {tuple(k8.shape)}")
-        if tuple(v8.shape) != (B, H, n // BLOCK, D, BLOCK):
-            raise ValueError(f"v8 must be {(B, H, n // BLOCK, D, BLOCK)}, got {tuple(v8.shape)}")
-        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            if tuple(t.shape) != (B, H, n // BLOCK) or t.dtype != torch.float32:
-                raise ValueError(f"{name} must be fp32 {(B, H, n // BLOCK)}, got {t.dtype} {tuple(t.shape)}")
+        if v8.shape != (B, H, nb, D, BLOCK):
+            raise ValueError(f"v8 must be {(B, H, nb, D, BLOCK)}, got {tuple(v8.shape)}")
         if k8.dtype != _E4M3 or v8.dtype != _E4M3:
             raise ValueError(f"k8 and v8 must be {_E4M3}, got {k8.dtype} and {v8.dtype}")
-        if not all(t.is_contiguous() for t in (k8, v8, k_scale, v_scale)) or k8.data_ptr() % 16 or v8.data_ptr() % 16:
+        if (k_scale.shape != (B, H, nb) or v_scale.shape != (B, H, nb)
+                or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32):
+            raise ValueError(f"k_scale and v_scale must be fp32 {(B, H, nb)}, got {k_scale.dtype} {tuple(k_scale.shape)} "
+                             f"and {v_scale.dtype} {tuple(v_scale.shape)}")
+        kp, vp = k8.data_ptr(), v8.data_ptr()
+        if ((kp | vp) % 16 or not k8.is_contiguous() or not v8.is_contiguous() or not k_scale.is_contiguous()
+                or not v_scale.is_contiguous()):
             raise ValueError("a cache's tensors must be contiguous, k8 and v8 on 16-byte boundaries")
         self.k8, self.v8, self.k_scale, self.v_scale = k8, v8, k_scale, v_scale
-        self._c = _lib.Cache8(k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, H, n, D)
+        self._c = _lib.Cache8(kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), B, H, n, D)
 
     @classmethod
     def empty(cls, batch: int, heads: int, capacity: int, head_dim: int, device=None) -> "KVCache8":
@@ -78,7 +83,8 @@ class KVCache8:
     @property
     def shape(self) -> tuple[int, int, int, int]:
         """(batch, heads, capacity, head_dim)."""
-        return tuple(self.k8.shape)
+        c = self._c
+        return c.B, c.H, c.capacity, c.D
 
     @property
     def capacity(self) -> int:
@@ -118,7 +124,7 @@ class KVCache8:
 def _ints(x: Ints, name: str, B: int, device: torch.device, lo: int, hi: int) -> torch.Tensor:
     """``x`` as the int32 ``[B]`` that the kernels read."""
     if isinstance(x, torch.Tensor):
-        if x.dtype != torch.int32 or tuple(x.shape) != (B,) or x.device != device:
+        if x.dtype != torch.int32 or x.shape != (B,) or x.device != device:
             raise ValueError(f"{name} must be an int or int32 [{B}] on {device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
         return x.contiguous()
     x = int(x)
@@ -128,8 +134,9 @@ def _ints(x: Ints, name: str, B: int, device: torch.device, lo: int, hi: int) ->
 
 
 def _no_grad(what: str, *ts: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    for t in ts:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start: Ints,
@@ -147,10 +154,10 @@ def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start: Ints,
     _require_device(cache.k8, k, v)
     _no_grad("cache_append", k, v)
     B, H, n, D = cache.shape
-    if k.dim() != 4 or k.shape != v.shape or k.shape[:2] != (B, H) or k.shape[3] != D or k.dtype != v.dtype:
+    S = k.shape[2] if k.dim() == 4 else -1
+    if k.shape != (B, H, S, D) or v.shape != (B, H, S, D) or k.dtype != v.dtype:
         raise ValueError(f"k, v must be [{B}, {H}, S, {D}] of one dtype, got {tuple(k.shape)} {k.dtype}, "
                          f"{tuple(v.shape)} {v.dtype}")
-    S = k.shape[2]
     code = _dtype_code(k)
     if S > n:
         raise ValueError(f"{S} rows for a cache of {n} tokens")
@@ -189,6 +196,11 @@ def _queries(what, q, cache, lengths, q_lens, sm_scale, max_len):
     return lengths, q_lens, sm_scale, max_len
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace(entry: str, Hq: int, S: int, B: int, H: int, n: int, D: int, max_len: int) -> int:
+    return getattr(_lib.load(), entry)(Hq, S, _lib.Cache8(None, None, None, None, B, H, n, D), max_len)
+
+
 def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens: Optional[Ints] = None,
                      causal: bool = False, sm_scale: Optional[float] = None, max_len: Optional[int] = None,
                      out: Optional[torch.Tensor] = None, return_lse: bool = False):
@@ -225,7 +237,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
     q, qs = rows_of(q, "q")
     to, os = rows_of(out, "out")  # a copy where out's rows cannot be written in place
     lib = _lib.load()
-    size = lib.lcv_bsa_cached_attn_workspace_bytes(Hq, S, cache._c, max_len)
+    size = _workspace("lcv_bsa_cached_attn_workspace_bytes", Hq, S, *cache.shape, max_len)
     ws = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
     with on_device(q):
         st = lib.lcv_bsa_cached_attn(q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._c, lengths.data_ptr(),
@@ -269,7 +281,7 @@ def attention_weights(q: torch.Tensor, cache: KVCache8, lengths: Ints, lse: torc
     lse = lse.contiguous()
     weights = None if weights is None else weights.contiguous()
     lib = _lib.load()
-    size = lib.lcv_bsa_attention_weights_workspace_bytes(Hq, S, cache._c, max_len)
+    size = _workspace("lcv_bsa_attention_weights_workspace_bytes", Hq, S, *cache.shape, max_len)
     ws = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
     with on_device(q):
         st = lib.lcv_bsa_attention_weights(

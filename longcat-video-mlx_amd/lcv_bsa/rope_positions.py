@@ -12,7 +12,8 @@ positions keep theirs.
 from __future__ import annotations
 
 import ctypes
-from typing import Sequence
+import functools
+from typing import Optional, Sequence
 
 import torch
 
@@ -28,13 +29,15 @@ _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 class on_device:
     """Makes ``t``'s device the current one for a launch (nothing where it is)."""
 
+    __slots__ = ("index", "before")
+
     def __init__(self, t: torch.Tensor):
-        self.index, self.before = t.device.index, None
+        self.index = t.device.index
 
     def __enter__(self):
         now = torch.cuda.current_device()
-        if now != self.index:
-            self.before = now
+        self.before = None if now == self.index else now
+        if self.before is not None:
             torch.cuda.set_device(self.index)
 
     def __exit__(self, *exc):
@@ -48,11 +51,12 @@ def rows_of(t: torch.Tensor, name: str) -> tuple[torch.Tensor, _lib.Strides]:
     of dimensions of size one put right)."""
     if t.dim() != 4:
         raise ValueError(f"{name} must be [B, H, S, D], got shape {tuple(t.shape)}")
-    D, vec = t.shape[3], 16 // t.element_size()
-    sb, sh, ss = (st if n > 1 else D for st, n in zip(t.stride(), t.shape[:3]))
-    if (t.stride(3) != 1 and D > 1) or ss < D or (sb | sh | ss) % vec or t.data_ptr() % 16:
+    B, H, S, D = t.shape
+    sb, sh, ss, sd = t.stride()
+    sb, sh, ss = sb if B > 1 else D, sh if H > 1 else D, ss if S > 1 else D
+    if (sd != 1 and D > 1) or ss < D or (sb | sh | ss) * t.element_size() % 16 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-        sb, sh, ss = (st if n > 1 else D for st, n in zip(t.stride(), t.shape[:3]))
+        return t, _lib.Strides(H * S * D, S * D, D)
     return t, _lib.Strides(sb, sh, ss)
 
 
@@ -63,21 +67,37 @@ def grid_positions(grid: Sequence[int], first: Sequence[int] = (0, 0, 0), device
     return torch.stack(torch.meshgrid(*axes, indexing="ij"), -1).reshape(-1, len(axes))
 
 
-def _rotate(x: torch.Tensor, positions: torch.Tensor, dims: Sequence[int], base: float, inverse: bool) -> torch.Tensor:
+@functools.lru_cache(maxsize=256)
+def _split(D: int, axes: int, dims: Optional[tuple]):
+    """The axes' dims (checked; None: the default split) as the entry point reads them."""
+    if D % 8 or not 8 <= D <= 256:
+        raise ValueError(f"rope_nd supports head dims that are multiples of 8 up to 256 (got {D})")
+    if axes < 1:
+        raise ValueError("positions need at least one axis")
+    if dims is None:
+        dims = rope_dims(D) if axes == 3 else (D // axes,) * axes
+    dims = tuple(int(d) for d in dims)
+    if len(dims) != axes or min(dims) < 2 or any(d % 2 for d in dims) or sum(dims) != D:
+        raise ValueError(f"dims must be {axes} even numbers that sum to {D}, got {dims}")
+    return (ctypes.c_int64 * axes)(*dims)
+
+
+def _rotate(x: torch.Tensor, positions: torch.Tensor, dims, base: float, inverse: bool) -> torch.Tensor:
     B, H, S, D = x.shape
     out = torch.empty_like(x)
     if not x.numel():
         return out
-    if out.stride(3) != 1 or out.stride(2) < D:  # x itself is not dense
+    sb, sh, ss, sd = out.stride()
+    if sd != 1 or ss < D:  # x itself is not dense
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        sb, sh, ss, sd = out.stride()
     x, xs = rows_of(x, "x")
-    os = _lib.Strides(*(st if n > 1 else D for st, n in zip(out.stride(), out.shape[:3])))
-    shared = positions.dim() == 2 or positions.shape[0] == 1
+    ps = positions.stride()
     with on_device(x):
         st = _lib.load().lcv_bsa_rope_nd(
             x.data_ptr(), _dtype_code(x), B, H, S, D, xs, positions.data_ptr(), _POSITION_TYPES[positions.dtype],
-            0 if shared else positions.stride(0), positions.stride(-2), (ctypes.c_int64 * len(dims))(*dims), len(dims),
-            base, int(inverse), out.data_ptr(), os, _stream(x))
+            ps[0] if len(ps) == 3 and positions.shape[0] > 1 else 0, ps[-2], dims, len(dims), base, inverse,
+            out.data_ptr(), _lib.Strides(sb if B > 1 else D, sh if H > 1 else D, ss if S > 1 else D), _stream(x))
     _lib.check(st, "rope_nd")
     return out
 
@@ -92,10 +112,11 @@ class _RopeNd(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         dims, base, inverse = ctx.how
-        return _RopeNd.apply(g, *ctx.saved_tensors, dims, base, not inverse), None, None, None, None
+        turn = _RopeNd.apply if torch.is_grad_enabled() else _rotate  # a second derivative is wanted, or not
+        return turn(g, *ctx.saved_tensors, dims, base, not inverse), None, None, None, None
 
 
-def rope_nd(x: torch.Tensor, positions: torch.Tensor, dims: Sequence[int] | None = None, *,
+def rope_nd(x: torch.Tensor, positions: torch.Tensor, dims: Optional[Sequence[int]] = None, *,
             base: float = BASE) -> torch.Tensor:
     """Rotates ``x`` ``[B, H, S, D]`` (fp16, bf16, fp32; D a multiple of 8 up to
     256; any strides) to its tokens' ``positions`` ``[S, axes]`` or ``[B, S, axes]``
@@ -113,19 +134,12 @@ def rope_nd(x: torch.Tensor, positions: torch.Tensor, dims: Sequence[int] | None
         raise ValueError(f"positions must be [{S}, axes] or [{B} or 1, {S}, axes], got {tuple(positions.shape)}")
     if positions.dtype not in _POSITION_TYPES:
         raise ValueError(f"positions must be int32, int64 or float32, got {positions.dtype}")
-    axes = positions.shape[-1]
-    if axes < 1:
-        raise ValueError("positions need at least one axis")
-    if D % 8 or not 8 <= D <= 256:
-        raise ValueError(f"rope_nd supports head dims that are multiples of 8 up to 256 (got {D})")
-    if dims is None:
-        dims = rope_dims(D) if axes == 3 else (D // axes,) * axes
-    dims = tuple(int(d) for d in dims)
-    if len(dims) != axes or min(dims) < 2 or any(d % 2 for d in dims) or sum(dims) != D:
-        raise ValueError(f"dims must be {axes} even numbers that sum to {D}, got {dims}")
-    positions = positions.detach()
-    if positions.stride(-1) != 1 or any(st < 0 for st in positions.stride()):
+    split = _split(D, positions.shape[-1], None if dims is None else tuple(dims))
+    if positions.requires_grad:
+        positions = positions.detach()
+    ps = positions.stride()
+    if ps[-1] != 1 or min(ps) < 0:
         positions = positions.contiguous()
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _RopeNd.apply(x, positions, dims, float(base), False)
-    return _rotate(x, positions, dims, float(base), False)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _RopeNd.apply(x, positions, split, float(base), False)
+    return _rotate(x, positions, split, float(base), False)

@@ -203,6 +203,8 @@ CASES = [
     (2, 3, 3, 64, 130, 448, [448, 1], [130, 130], False),
     (1, 8, 1, 128, 40, 640, [600], None, False),
     (2, 2, 2, 128, 300, 704, [700, 0], [1, 300], True),
+    (70, 1, 1, 64, 1, 1280, [(37 * i * i) % 1281 for i in range(70)], None, False),  # more items than lanes, parts of 8 blocks
+    (3, 3, 3, 64, 60, 1344, [1300, 30, 0], [60, 60, 5], True),
 ]
 
 
