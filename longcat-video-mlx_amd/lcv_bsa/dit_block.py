@@ -430,8 +430,10 @@ class LongCatSingleStreamBlock(nn.Module):
         _, x_m = residual_norm(x, frames=T, shift=shift_msa, scale=scale_msa, eps=self.mod_norm_attn.eps)
         x_s, new_kv = self._self_attn(x_m, latent_shape, num_cond_latents, return_kv, kv_cache)
         pre = self.pre_crs_attn_norm
-        x, xn = residual_norm(x, x_s, gate_msa, frames=T, weight=pre.weight, bias=pre.bias, eps=pre.eps,
-                              norm=not skip_crs_attn)
+        if skip_crs_attn:
+            x, _ = residual_norm(x, x_s, gate_msa, frames=T, norm=False)
+        else:
+            x, xn = residual_norm(x, x_s, gate_msa, frames=T, weight=pre.weight, bias=pre.bias, eps=pre.eps)
         if not skip_crs_attn:
             ncl_cross = None if kv_cache is not None else num_cond_latents
             c = self.cross_attn(xn, y, y_seqlen, ncl_cross, latent_shape)
