@@ -27,8 +27,10 @@ import torch.nn.functional as F
 from .attention import BSAAttention, dense_attention, validate_backend
 from .block_ops import adaln_modulation, head_rms_norm, plain_tensors, residual_norm, swiglu, text_attention, unwatched
 from .block_sparse_attention import bsa_attention
+from .kv_cache import KVCache8, cache_append, cached_attention
 from .prepare import prepare_qk, prepare_qkv
-from .rope_3d import rope_3d
+from .rope_3d import rope_3d, rope_dims
+from .rope_positions import grid_positions, rope_nd
 from .shape_policy import bsa_geometry
 
 __all__ = [
@@ -136,7 +138,11 @@ class Attention(nn.Module, BSAAttention):
     straight into the ``[B, N, H, D]`` layout of the output projection; around
     a KV cache (returned, or continued) ``prepare_qkv`` does the same where no
     gradient is wanted through the cache.  A ``ValueError`` anywhere on that
-    path falls back to the reference's unfused sequence."""
+    path falls back to the reference's unfused sequence.
+
+    ``kv_cache_8bit = True`` keeps the cache that ``return_kv`` asks for in 8 bits: a
+    pair of a ``KVCache8`` (keys after RoPE; half the memory of the reference's, without
+    a gradient) and the number of its tokens; ``forward_with_kv_cache`` takes either kind."""
 
     def __init__(self, dim: int, num_heads: int, **kw):
         nn.Module.__init__(self)
@@ -147,6 +153,7 @@ class Attention(nn.Module, BSAAttention):
         self.proj = nn.Linear(dim, dim, **kw)
         self.bsa_shape_policy: str = "reference"
         self.bsa_cond_noise: bool = False
+        self.kv_cache_8bit: bool = False
         self.keep_indices: bool = False          # store the last routing per branch (tests)
         self.last_indices: dict = {}
         self.last_paths: dict = {}
@@ -197,14 +204,15 @@ class Attention(nn.Module, BSAAttention):
         qkv = self.qkv(x).view(B, N, 3, H, D)
         q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
         o = torch.empty((B, N, H, D), dtype=x.dtype, device=x.device)
+        eight = return_kv and self.kv_cache_8bit
         if (self.enable_bsa and shape is not None
-                and (not return_kv or self._cache_fusible(qkv))):
+                and (not return_kv or eight or self._cache_fusible(qkv))):
             validate_backend(self.bsa_backend)
             geom = bsa_geometry(shape, self.bsa_chunk_thw, self.bsa_shape_policy)
             if geom is not None:
                 weights = dict(q_weight=self.q_norm.weight, k_weight=self.k_norm.weight, eps=self.q_norm.eps)
                 try:
-                    if return_kv:
+                    if return_kv and not eight:
                         kn = torch.empty((B, N, H, D), dtype=k.dtype, device=k.device).transpose(1, 2)
                         qp, kp, _, qb, kb = prepare_qkv(q, k, None, shape, geom[0], geom[0], geom[1], k_norm=kn,
                                                         **weights)
@@ -214,14 +222,17 @@ class Attention(nn.Module, BSAAttention):
                         self._split(qp, kp, v, shape, ncl, o)
                     else:
                         self._attend("all", qp, kp, v, shape, means=(qb, kb), out=o.transpose(1, 2))
+                    cache = self._cache8(kp, v) if eight else (kn, v) if return_kv else None
                     out = self.proj(o.view(B, N, C))
-                    return (out, (kn, v)) if return_kv else out
+                    return (out, cache) if return_kv else out
                 except ValueError:
                     self.last_indices, self.last_paths = {}, {}
         # The reference's sequence: norms, (cache,) RoPE, then BSA-or-dense.
         q, k = self.q_norm(q), self.k_norm(k)
         cache = (k, v)
         q, k = rope_3d(q, k, tuple(shape))
+        if eight:
+            cache = self._cache8(k, v)
         if ncl > 0:
             self._split(q, k, v, shape, ncl, o)
         else:
@@ -234,6 +245,37 @@ class Attention(nn.Module, BSAAttention):
         differentiates or traces through them, and both round and weigh alike."""
         return (plain_rms_norms(self.q_norm, self.k_norm) and self.q_norm.eps == self.k_norm.eps
                 and plain_tensors(*tensors, self.q_norm.weight, self.k_norm.weight))
+
+    @staticmethod
+    def _cache8(k: torch.Tensor, v: torch.Tensor) -> tuple[KVCache8, int]:
+        """The 8-bit cache of rotated keys and values ``[B, H, N, D]``, and N."""
+        return cache_append(KVCache8.empty(*k.shape, device=k.device), k, v, 0), k.shape[2]
+
+    def _continue_8bit(self, x: torch.Tensor, shape: Sequence[int], ncl: int, cache: KVCache8,
+                       cached: int) -> torch.Tensor:
+        """The continuation from an 8-bit cache of ``ncl`` frames: the new tokens are
+        turned to their frames' positions and appended to a copy of it, and their
+        queries attend to all of it (densely, as the reference's do)."""
+        B, N, C = x.shape
+        H, D = self.num_heads, self.head_dim
+        T, Hl, Wl = (int(s) for s in shape)
+        b, h, n, d = cache.shape
+        if ncl <= 0 or N != T * Hl * Wl or b not in (1, B) or (h, d) != (H, D) or not cached == ncl * Hl * Wl <= n:
+            raise ValueError(f"an 8-bit cache {cache.shape} of {cached} tokens does not hold {ncl} frames of {Hl} x {Wl} "
+                             f"before {N} new tokens of {B} items, {H} heads of {D}")
+        q, k, v = (t.transpose(1, 2) for t in self.qkv(x).view(B, N, 3, H, D).unbind(2))
+        if D in (64, 128) and self._cache_fusible(q, k):
+            q, k = (head_rms_norm(t, m.weight, m.eps) for t, m in ((q, self.q_norm), (k, self.k_norm)))
+        else:
+            q, k = self.q_norm(q), self.k_norm(k)
+        positions = grid_positions((T, Hl, Wl), (ncl, 0, 0), x.device)
+        q, k = (rope_nd(t, positions, rope_dims(D)) for t in (q, k))
+        cache = cache_append(cache.extended(max(n, cached + N), B), k, v, cached)
+        o = torch.empty((B, N, H, D), dtype=x.dtype, device=x.device)
+        cached_attention(q, cache, cached + N, sm_scale=self.scale, out=o.transpose(1, 2))
+        self.last_indices, self.last_paths = {}, {"noise": "dense"}
+        self.last_path = "dense"
+        return self.proj(o.view(B, N, C))
 
     def _continue_fused(self, q, k, v, x, shape, ncl, kv_cache):
         """The continuation with BSA over cached + new keys, from one
@@ -267,7 +309,10 @@ class Attention(nn.Module, BSAAttention):
         """Chunked continuation (attention.py:235-275): fresh k / v appended to
         the cached (normed, un-rotated) ones; with conditioning latents RoPE
         runs over the extended grid (q zero-padded to align positions); the
-        noise queries then attend to all keys."""
+        noise queries then attend to all keys.  From an 8-bit cache the keys are
+        rotated already, so it needs the conditioning latents."""
+        if isinstance(kv_cache[0], KVCache8):
+            return self._continue_8bit(x, shape, int(num_cond_latents or 0), *kv_cache)
         B, N, C = x.shape
         H, D = self.num_heads, self.head_dim
         qkv = self.qkv(x).view(B, N, 3, H, D)

@@ -28,6 +28,10 @@ def _x(device, B, frames, C, dtype=torch.bfloat16, seed=1):
     return torch.randn(B, frames * GRID[1] * GRID[2], C, generator=g, device=device).to(dtype)
 
 
+def _parts(cache):
+    return cache.k8.view(torch.uint8), cache.v8.view(torch.uint8), cache.k_scale, cache.v_scale
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("batch", [1, 2])
@@ -42,14 +46,14 @@ def test_continuation(device, dtype, dim, batch):
         m.kv_cache_8bit = False
         out, plain = m(first, GRID, return_kv=True)
         assert torch.equal(out8, out)
-        assert cache.shape == (1, 2, 128, dim)
+        assert cache[0].shape == (1, 2, 128, dim) and cache[1] == 84
         want = m.forward_with_kv_cache(more, (3,) + GRID[1:], 2, plain).float()
-        before = [t.clone() for t in (cache.k8.view(torch.uint8), cache.v8.view(torch.uint8), cache.k_scale, cache.v_scale)]
+        before = [t.clone() for t in _parts(cache[0])]
         got = m.forward_with_kv_cache(more, (3,) + GRID[1:], 2, cache)
         off = (got.float() - want).norm() / (want - m.proj.bias.float()).norm()
         assert float(off) < 2.0 ** -4
         # a step of a denoising loop leaves the cache as it was, and the next gives the same
-        for a, b in zip(before, (cache.k8.view(torch.uint8), cache.v8.view(torch.uint8), cache.k_scale, cache.v_scale)):
+        for a, b in zip(before, _parts(cache[0])):
             assert torch.equal(a, b)
         m.forward_with_kv_cache(100 * more, (3,) + GRID[1:], 2, cache)
         assert torch.equal(got, m.forward_with_kv_cache(more, (3,) + GRID[1:], 2, cache))
@@ -62,7 +66,7 @@ def test_keys_are_rotated_once(device):
     m = _layer(device)
     with torch.no_grad():
         x = _x(device, 1, 2, 256)
-        _, cache = m(x, GRID, return_kv=True)
+        _, (cache, _) = m(x, GRID, return_kv=True)
         m.kv_cache_8bit = False
         _, (k, v) = m(x, GRID, return_kv=True)
         _, k = rope_3d(k, k, GRID)
@@ -78,10 +82,10 @@ def test_with_block_sparse_attention(device):
     m = _layer(device, bsa=True)
     with torch.no_grad():
         x = torch.randn(1, 128, 256, device=device, generator=torch.Generator(device=device).manual_seed(3)).to(torch.bfloat16)
-        _, cache = m(x, grid, return_kv=True)
+        _, (cache, _) = m(x, grid, return_kv=True)
         assert m.last_path == "bsa"
         m.enable_bsa = False
-        _, plain = m(x, grid, return_kv=True)
+        _, (plain, _) = m(x, grid, return_kv=True)
         (k, v), (k0, v0) = cache.dequantize(), plain.dequantize()
         assert torch.equal(v, v0)
         # k's norm and rotation round in other places: a step of bf16, then a step of e4m3
