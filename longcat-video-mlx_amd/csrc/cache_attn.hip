@@ -730,7 +730,7 @@ Kind kind_of(const CacheAttn& a) {
 // The walks are split where there are too few to fill the chip and to even out items of
 // different lengths, into parts of at least 8 blocks; a short history is walked at once.
 constexpr int64_t kFewParts = 1024, kFewBlocks = 8, kOnePart = 16;
-constexpr int64_t kManyParts = 2304, kManyBlocks = 8;
+constexpr int64_t kManyParts = 512, kManyBlocks = 6, kManyOnePart = 8;
 constexpr int64_t kJoinRows = 4096;
 
 Parts plan(const CacheAttn& a) {
@@ -741,11 +741,11 @@ Parts plan(const CacheAttn& a) {
   const int64_t walks = (int64_t)a.c.B * a.c.H * ((rows + wide - 1) / wide);
   p.tiles = (int)((rows + wide - 1) / wide * (wide / 16));
   int64_t per = blocks;
-  if (kind == kMany) {
+  if (kind == kMany && blocks > kManyOnePart) {
     const int64_t splits = (kManyParts + walks - 1) / walks;
     per = (blocks + splits - 1) / splits;
     if (per < kManyBlocks) per = kManyBlocks;
-  } else if (blocks > kOnePart) {
+  } else if (kind != kMany && blocks > kOnePart) {
     const int64_t want = (blocks * walks + kFewParts - 1) / kFewParts;
     per = (want + 3) / 4 * 4;
     if (per < kFewBlocks) per = kFewBlocks;

@@ -5,7 +5,7 @@
 // order of the floats (NaN below everything), held in LDS, and a search for the number T
 // of the last token to stay (count above T < want <= count from T on).  A round sorts the
 // candidates into 4096 bins of the interval [a, z) by a shift, and goes on in the bin where
-// the count passes `want`: three rounds at most, whatever the weights.  As soon as 512 are
+// the count passes `want`: three rounds at most, whatever the weights.  As soon as 32 are
 // left they are compared with one another.  Each wave holds a run of tokens, so one
 // exchange of the waves' counts places every kept token; equal weights at T stay from the
 // lowest token on.
@@ -30,7 +30,7 @@ constexpr uint64_t kKeysEnd = 0xff800001;  // past infinity's
 
 constexpr int kRankThreads = 1024, kRankWaves = kRankThreads / 64;
 constexpr int kBins = 4096;
-constexpr uint32_t kLast = 512;
+constexpr uint32_t kLast = 32;
 
 // N: keys that LDS holds, or 0 where the weights are read anew at each pass.  (In
 // registers the loops over them would be unrolled, and a launch that runs each

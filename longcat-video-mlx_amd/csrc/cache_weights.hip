@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void add_parts_kernel(const float* w_in, const
   w_out[i] = (w_in ? w_in[i] : 0.0f) + sum;
 }
 
-constexpr int kFewRows = 96;
+constexpr int kFewRows = 64;
 
 // The rows are split over workgroups where the keys are too few to fill the chip.
 int row_splits(const CacheAttn& a) {

@@ -49,11 +49,11 @@ __global__ __launch_bounds__(256) void rope_nd_kernel(RopeNd r, Share w) {
   __syncthreads();
   const T* x = reinterpret_cast<const T*>(r.x.ptr) + (int64_t)b * r.x.sb + (int64_t)s0 * r.x.ss + (int64_t)h0 * r.x.sh;
   T* y = reinterpret_cast<T*>(const_cast<void*>(r.y.ptr)) + (int64_t)b * r.y.sb + (int64_t)s0 * r.y.ss + (int64_t)h0 * r.y.sh;
-  const int chunks = 2 * r.pairs / kVec, total = tokens * heads * chunks;
+  const int chunks = 2 * r.pairs / kVec;
   // The inner count is a full part's, so that one divisor serves; what it adds is skipped.
   const int inner = w.by_token ? w.heads : w.tokens, outer = w.by_token ? tokens : heads;
   const int all = outer * inner * chunks;
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = 2;
   for (int i0 = tid; i0 < all; i0 += 256 * kUnroll) {
     u32x4 v[kUnroll];
     int64_t to[kUnroll];
@@ -95,6 +95,7 @@ hipError_t launch(const RopeNd& r, hipStream_t stream) {
   // heads split the same way (their angles are formed anew).
   const int chunks = 2 * r.pairs / kVec;
   w.tokens = kMaxAngles / r.pairs < 16 ? kMaxAngles / r.pairs : 16;
+  while (w.tokens > 1 && (int64_t)w.tokens * r.H * chunks > 1024) w.tokens /= 2;
   while (w.tokens > 1 && (int64_t)r.B * ((r.S + w.tokens - 1) / w.tokens) < 1024) w.tokens /= 2;
   w.heads = r.H;
   while (w.heads > 1 && (int64_t)r.B * ((r.S + w.tokens - 1) / w.tokens) * ((r.H + w.heads - 1) / w.heads) < 512 &&
