@@ -102,11 +102,12 @@ void many_weights_kernel(CacheAttn a, const float* w_in, float* w_out, float* pa
 
   const int wid = xcd_linear_work_id(blockIdx.x, gridDim.x);
   const int quads = (a.c.nb + 3) / 4;
-  const int bh = wid / (quads * splits), split = wid / quads % splits;
+  // The items of a head next to one another: an XCD's share is not one item's, which may be short.
+  const int kvh = wid / (quads * splits) / a.c.B, b = wid / (quads * splits) % a.c.B, bh = b * a.c.H + kvh;
+  const int split = wid / quads % splits;
   const int lane = threadIdx.x % 64, G = lane / 16, gi = lane % 16;
   const int wave = uniform_i32(threadIdx.x / 64);
   const int j = wid % quads * 4 + wave;
-  const int b = bh / a.c.H, kvh = bh - b * a.c.H;
   const Lens n = item_lens(a, b);
   const int64_t block = (int64_t)bh * a.c.nb + j;
   const bool mine = j < a.c.nb && 64 * j < n.len;  // wave-uniform
