@@ -355,6 +355,58 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttn a, Parts p, int wid
   if (a.lse && lane == 0) a.lse[lse_at(a, b, kvh, r)] = empty ? kNegInf : (top + __builtin_log2f(lsum)) * kLn2;
 }
 
+constexpr int kSorted = 8;
+
+// Which tile of 128 rows of which item a workgroup takes: the r-th of a key head's.
+struct Turn {
+  int b, tile;
+};
+
+// Items next to one another, of each the longest walk first.  A CU's workgroups, 32 apart,
+// are not all one item's.
+__device__ __forceinline__ Turn in_turn(const CacheAttn& a, int tiles, int r) {
+  const int b = (r + r / a.c.B * a.c.B / 32) % a.c.B, at = r / a.c.B;
+  return {b, a.causal ? tiles - 1 - at : at};
+}
+
+// The longest walk of all items first (up to kSorted of them).  Lane b holds item b's
+// lengths; the walk of the r-th is the largest x that more than r tiles reach, looked for
+// 64 numbers at a time.
+__device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) {
+  const int lane = threadIdx.x % 64;
+  const Lens mine = item_lens(a, lane < a.c.B ? lane : 0);
+  auto item = [&](int b) { return Lens{__builtin_amdgcn_readlane(mine.len, b), __builtin_amdgcn_readlane(mine.ql, b)}; };
+  auto real = [&](const Lens& n) { return (n.ql * a.group + 127) / 128; };  // tiles with queries
+  auto reaching = [&](const Lens& n, int x) {  // how many of the item's tiles walk x blocks or more
+    if (x == 0) return tiles;
+    if (64 * (x - 1) >= n.len || n.ql == 0) return 0;
+    const int t = real(n), i = 64 * (x - 1) - (n.len - n.ql);  // the first query to see the x-th block
+    const int first = a.causal && i > 0 ? i * a.group / 128 : 0;
+    return t - (first < t ? first : t - 1);
+  };
+  int lo = 0, hi = (a.max_len + 63) / 64 + 1;  // more than r reach lo, not so hi
+  while (hi - lo > 1) {                        // wave-uniform
+    const int step = (hi - lo + 64) / 65, x = lo + (lane + 1) * step;
+    int all = 0;
+    for (int b = 0; b < a.c.B; ++b) all += x < hi ? reaching(item(b), x) : 0;
+    const int n = __popcll(__ballot(all > r));
+    lo += n * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  // Lane b: the tiles of item b that walk lo blocks, behind those of the items before.
+  const int from = reaching(mine, lo + 1), n = lane < a.c.B ? reaching(mine, lo) - from : 0;
+  int longer = lane < a.c.B ? from : 0, upto = n;
+  for (int o = 1; o < a.c.B; o <<= 1) {
+    longer += __shfl_xor(longer, o);
+    const int x = __shfl_up(upto, o);
+    upto += lane >= o ? x : 0;
+  }
+  r -= __builtin_amdgcn_readlane(longer, 0);
+  const int b = __builtin_ctzll(__ballot(upto > r));
+  const int at = __builtin_amdgcn_readlane(from + n - upto, b) + r, t = __builtin_amdgcn_readlane(real(mine), b);
+  return {b, at < t ? t - 1 - at : at};  // the tiles without queries last
+}
+
 // Many rows: one workgroup of four waves takes 128 rows of one key head, wave w rows
 // 32 w .. 32 w + 31, and walks a part of the blocks.  A block's 8 KB of keys and 8 KB
 // of values (D = 128) go straight from memory into a ring of three LDS slots, two
@@ -391,16 +443,12 @@ void many_rows_kernel(CacheAttn a, Parts p) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[3 * kSlot];
   static_assert(3 * kSlot >= kRows * 2 * D, "the ring stages the output rows");
 
-  // Work ids: batch items next to one another, then the tiles of a head, its parts, the
-  // heads.  Items of different lengths then share an XCD's time.
   const int wid = xcd_linear_work_id(blockIdx.x, gridDim.x);
-  const int turn = wid / a.c.B * a.c.B / 32;  // a CU's workgroups, 32 apart, are not all one item's
-  const int b = (wid % a.c.B + turn) % a.c.B;
   const int tiles = p.tiles / 8;  // of 128 rows
-  const int at = wid / a.c.B % tiles;
-  const int tile = a.causal ? tiles - 1 - at : at;  // the longest walks first
-  const int split = wid / (a.c.B * tiles) % p.splits;
+  const int of_head = wid % (a.c.B * tiles), split = wid / (a.c.B * tiles) % p.splits;
   const int kvh = wid / (a.c.B * tiles * p.splits);
+  const Turn turn = a.c.B > 1 && a.c.B <= kSorted && p.splits == 1 ? by_length(a, tiles, of_head) : in_turn(a, tiles, of_head);
+  const int b = turn.b, tile = turn.tile;
   const int bh = b * a.c.H + kvh;
   const int tid = threadIdx.x, lane = tid % 64, G = lane / 16, gi = lane % 16;
   const int wave = uniform_i32(tid / 64);

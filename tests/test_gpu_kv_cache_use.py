@@ -271,3 +271,40 @@ def test_beyond_32_bits(device, S):
     got_v = c.v8.view(torch.uint8)[0, 1][at // 64, :, at % 64].view(e4m3).float() * c.v_scale[0, 1][at // 64][:, None]
     for x, y, scale in ((fk[0, 1, :200], got_k, few.k_scale), (fv[0, 1, :200], got_v, few.v_scale)):
         assert bool(((x - y).abs() <= 2.0 ** -4 * y.abs() + 2.0 ** -10 * scale.max()).all())
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,q_lens", [
+    ([500, 0, 3, 129, 512], [300, 7, 0, 129, 1]),
+    ([64, 400], [300, 300]),  # item 0: queries before its first token
+    ([5, 70, 140, 200, 512, 1, 0, 333, 64], [5, 70, 100, 0, 300, 1, 2, 33, 64]),
+])
+def test_ragged_batches(device, lengths, q_lens, causal):
+    """Every row of every item is answered, whatever the order of the walks."""
+    from lcv_bsa import attention_weights, cached_attention
+
+    gen = _gen(device, len(lengths))
+    B, S = len(lengths), 300
+    c = _cache(gen, device, B, 2, 512, 64, stale=lengths)
+    q = _rows(gen, device, B, 4, S, 64, BF16)
+    out = torch.full((B, 4, S, 64), math.nan, dtype=BF16, device=device)
+    n, m = _ints(device, lengths), _ints(device, q_lens)
+    _, lse = cached_attention(q, c, n, q_lens=m, causal=causal, out=out, return_lse=True)
+    want, want_lse, tol, tol_lse, probs, tol_p = R.attention(q, c, lengths, q_lens, causal)
+    _within(out, want, tol)
+    _within(lse, want_lse, tol_lse)
+    given, tol_w = R.weights(probs, tol_p, 2)
+    _within(attention_weights(q, c, n, lse, q_lens=m, causal=causal), given, tol_w + 2.0 ** -23 * given)
+
+
+def test_rotary_rows_beyond_32_bits(device):
+    """2^31 elements and more: the last heads' rows as on their own."""
+    from lcv_bsa import rope_nd
+
+    x = torch.zeros(1, 40, 1 << 20, 64, dtype=F16, device=device)
+    x[:, -2:].normal_(generator=_gen(device, 2))
+    pos = torch.arange(1 << 20, device=device)[:, None]
+    want = rope_nd(x[:, -2:], pos)
+    assert torch.equal(rope_nd(x, pos)[:, -2:], want)
+    turned = x.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(rope_nd(turned, pos)[:, -2:], want)
