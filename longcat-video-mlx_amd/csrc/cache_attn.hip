@@ -39,16 +39,37 @@ __device__ __forceinline__ Reach reach(const CacheAttn& a, const Lens& n, int r0
   return {visible(a, n, i1), least > 0 ? least : 1};
 }
 
-// How the walk over the blocks is split: parts of `per` blocks, at most `splits`.  Their
-// sums and maxima lie in the workspace by (split, key head, 16 rows).
+// How the walk over the blocks is split.  Many rows: into parts of `per` blocks, at most
+// `splits` of an item, part s of item b in slot s B + b.  Few rows: per is 0, the parts go
+// by the lengths (few_per), at most `splits` of all items, which take the slots one after
+// another.  A part's sums and maxima lie in the workspace by (slot, key head, 16 rows).
 struct Parts {
-  int32_t tiles;   // of 16 rows, of one key head
+  int32_t tiles;  // of 16 rows, of one key head
   int32_t splits, per;
-  float* o;        // [splits][B * H][tiles][16][D]
-  float* ml;       // [splits][B * H][tiles][16][2]
+  float* o;       // [slots][H][tiles][16][D]
+  float* ml;      // [slots][H][tiles][16][2]
+  int32_t* items; // [B][2], few rows: an item's first slot, the blocks of its parts
 };
-__device__ __forceinline__ int64_t part_at(const CacheAttn& a, const Parts& p, int split, int bh, int tile) {
-  return ((int64_t)split * a.c.B * a.c.H + bh) * p.tiles + tile;
+__device__ __forceinline__ int64_t part_at(const CacheAttn& a, const Parts& p, int slot, int kvh, int tile) {
+  return ((int64_t)slot * a.c.H + kvh) * p.tiles + tile;
+}
+
+__device__ __forceinline__ int item_blocks(const CacheAttn& a, int b) { return (item_lens(a, b).len + 63) / 64; }
+
+// Few rows: the blocks of a part, so that all items together, `walks` times each, make
+// about kFewParts parts.  Wave-uniform.
+constexpr int kFewParts = 512, kFewBlocks = 8, kOnePart = 16;
+__device__ __forceinline__ int few_per(const CacheAttn& a, int walks, int blocks) {  // blocks: item `lane`'s
+  for (int b = 64 + threadIdx.x % 64; b < a.c.B; b += 64) blocks += item_blocks(a, b);
+  for (int o = 1; o < 64 && o < a.c.B; o <<= 1) blocks += __shfl_xor(blocks, o);
+  const int64_t all = __builtin_amdgcn_readlane(blocks, 0);
+  const int per = (int)((all * walks + 4 * kFewParts - 1) / (4 * kFewParts) * 4);
+  return per < kFewBlocks ? kFewBlocks : per;
+}
+// An item's own: a short history is one part.
+__device__ __forceinline__ int item_per(int blocks, int per) { return blocks <= kOnePart ? kOnePart : per; }
+__device__ __forceinline__ int item_parts(int blocks, int per) {
+  return blocks <= kOnePart ? 1 : (blocks + per - 1) / per;
 }
 
 template <typename T>
@@ -88,13 +109,11 @@ void few_rows_kernel(CacheAttn a, Parts p) {
   const int u = slot / wide * kNumXcd + blockIdx.x % kNumXcd;
   const int lane = threadIdx.x % 64, G = lane / 16, gi = lane % 16;
   const int kvh = u % a.c.H;
-  int b = a.c.B == 1 ? 0 : -1, split = u / a.c.H;
+  const int slot_at = u / a.c.H;
+  const int blocks = lane < a.c.B ? item_blocks(a, lane) : 0, few = few_per(a, a.c.H * (p.tiles / NT), blocks);
+  int b = a.c.B == 1 ? 0 : -1, split = slot_at;
   for (int b0 = 0; b < 0 && b0 < a.c.B; b0 += 64) {  // wave-uniform
-    int parts = 0;
-    if (b0 + lane < a.c.B) {
-      const int len = item_lens(a, b0 + lane).len;
-      parts = len > 0 ? ((len + 63) / 64 + p.per - 1) / p.per : 1;
-    }
+    const int parts = b0 + lane < a.c.B ? item_parts(b0 == 0 ? blocks : item_blocks(a, b0 + lane), few) : 0;
     int upto = parts;
     for (int o = 1; o < 64 && o < a.c.B; o <<= 1) {
       const int x = __shfl_up(upto, o);
@@ -115,9 +134,11 @@ void few_rows_kernel(CacheAttn a, Parts p) {
   const Lens n = item_lens(a, b);
   const int rows = a.group * a.S;
   const Reach all = reach(a, n, 16 * tile, 16 * tile + 16 * NT);
-  const int nblk = (all.most + 63) / 64;
-  const int j0 = split * p.per;
-  const int j1 = j0 + p.per < nblk ? j0 + p.per : nblk;
+  const int nblk = (all.most + 63) / 64, per = item_per((n.len + 63) / 64, few);
+  if (p.items && split == 0 && kvh == 0 && tile == 0 && threadIdx.x == 0)
+    p.items[2 * b] = slot_at, p.items[2 * b + 1] = per;
+  const int j0 = split * per;
+  const int j1 = j0 + per < nblk ? j0 + per : nblk;
   if (split > 0 && j0 >= nblk) return;  // the first part of a tile always answers
 
   vec8 qf[NT][D / 32];
@@ -261,7 +282,7 @@ void few_rows_kernel(CacheAttn a, Parts p) {
     }
   }
   // The four waves' parts together: thread (row, 16th of D).
-  const bool last = nblk <= p.per;  // nothing to join
+  const bool last = nblk <= per;  // nothing to join
   const int row = threadIdx.x / 16, d0 = threadIdx.x % 16 * (D / 16);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -299,7 +320,7 @@ void few_rows_kernel(CacheAttn a, Parts p) {
       __builtin_memcpy(__builtin_assume_aligned(out_row<T>(a, b, kvh, r) + d0, 2 * D / 16), t, sizeof(t));
       if (a.lse && d0 == 0) a.lse[lse_at(a, b, kvh, r)] = empty ? kNegInf : (top + __builtin_log2f(lsum)) * kLn2;
     } else {
-      const int64_t at = part_at(a, p, split, bh, tile + nt);
+      const int64_t at = part_at(a, p, slot_at, kvh, tile + nt);
       __builtin_memcpy(__builtin_assume_aligned(p.o + at * (16 * D) + row * D + d0, 4 * D / 16), acc, sizeof(acc));
       if (d0 == 0) {
         p.ml[at * 32 + 2 * row] = top;
@@ -320,18 +341,23 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttn a, Parts p, int wid
   const int rows = a.group * a.S;
   const int r = (int)(id % rows), bh = (int)(id / rows);
   const int b = bh / a.c.H, kvh = bh - b * a.c.H;
+  int slot = b, step = a.c.B, per = p.per;
+  if (per == 0) {  // few rows: the items' parts one after another
+    slot = p.items[2 * b], per = p.items[2 * b + 1];
+    step = 1;
+  }
   const Lens n = item_lens(a, b);
   const int first = r / wide * wide;
   const int nblk = (reach(a, n, first, first + wide).most + 63) / 64;
-  if (nblk <= p.per) return;  // written already
-  const int parts = (nblk + p.per - 1) / p.per;
+  if (nblk <= per) return;  // written already
+  const int parts = (nblk + per - 1) / per;
   const int lane = threadIdx.x % THREADS;
-  const int64_t step = (int64_t)a.c.B * a.c.H * p.tiles;
-  const int64_t at = part_at(a, p, 0, bh, r / 16);
+  const int64_t stride = (int64_t)step * a.c.H * p.tiles;
+  const int64_t at = part_at(a, p, slot, kvh, r / 16);
   const float* ml = p.ml + at * 32 + 2 * (r % 16);
   const float* o = p.o + at * (16 * D) + r % 16 * D + lane * kN;
   float top = kNegInf;
-  for (int i = lane; i < parts; i += THREADS) top = __builtin_elementwise_maximum(top, ml[i * step * 32]);
+  for (int i = lane; i < parts; i += THREADS) top = __builtin_elementwise_maximum(top, ml[i * stride * 32]);
   for (int x = 1; x < THREADS; x <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, x));
   const float base = top == kNegInf ? 0.0f : top;
   float lsum = 0.0f, acc[kN];
@@ -339,10 +365,10 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttn a, Parts p, int wid
   for (int e = 0; e < kN; ++e) acc[e] = 0.0f;
 #pragma unroll 4
   for (int i = 0; i < parts; ++i) {
-    const float f = fast_exp2(ml[i * step * 32] - base);
-    lsum = __builtin_fmaf(ml[i * step * 32 + 1], f, lsum);
+    const float f = fast_exp2(ml[i * stride * 32] - base);
+    lsum = __builtin_fmaf(ml[i * stride * 32 + 1], f, lsum);
     float x[kN];
-    __builtin_memcpy(x, __builtin_assume_aligned(o + i * step * (16 * D), 4 * kN > 16 ? 16 : 4 * kN), sizeof(x));
+    __builtin_memcpy(x, __builtin_assume_aligned(o + i * stride * (16 * D), 4 * kN > 16 ? 16 : 4 * kN), sizeof(x));
 #pragma unroll
     for (int e = 0; e < kN; ++e) acc[e] = __builtin_fmaf(x[e], f, acc[e]);
   }
@@ -717,7 +743,7 @@ void many_rows_kernel(CacheAttn a, Parts p) {
   __syncthreads();  // the ring is free
 
   if (nblk > p.per) {
-    const int64_t part = part_at(a, p, split, bh, 8 * tile + 2 * wave);
+    const int64_t part = part_at(a, p, split * a.c.B + b, kvh, 8 * tile + 2 * wave);
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
       float* po = p.o + (part + qt) * (16 * D) + gi * D + 4 * G;
@@ -775,51 +801,59 @@ Kind kind_of(const CacheAttn& a) {
   return rows <= 16 ? kFew16 : rows <= kFewRows ? kFew32 : kMany;
 }
 
-// The walks are split where there are too few to fill the chip and to even out items of
-// different lengths, into parts of at least 8 blocks; a short history is walked at once.
-constexpr int64_t kFewParts = 1024, kFewBlocks = 8, kOnePart = 16;
 constexpr int64_t kManyParts = 512, kManyBlocks = 6, kManyOnePart = 8;
 constexpr int64_t kJoinRows = 4096;
+
+int wide_of(Kind kind) { return kind == kMany ? 128 : kind == kFew32 ? 32 : 16; }
 
 Parts plan(const CacheAttn& a) {
   Parts p{};
   const Kind kind = kind_of(a);
   const int64_t rows = (int64_t)a.group * a.S, blocks = ((int64_t)a.max_len + 63) / 64;
-  const int wide = kind == kMany ? 128 : kind == kFew32 ? 32 : 16;
-  const int64_t walks = (int64_t)a.c.B * a.c.H * ((rows + wide - 1) / wide);
+  const int wide = wide_of(kind);
+  const int64_t walks = (int64_t)a.c.H * ((rows + wide - 1) / wide);  // of an item
   p.tiles = (int)((rows + wide - 1) / wide * (wide / 16));
-  int64_t per = blocks;
-  if (kind == kMany && blocks > kManyOnePart) {
-    const int64_t splits = (kManyParts + walks - 1) / walks;
-    per = (blocks + splits - 1) / splits;
-    if (per < kManyBlocks) per = kManyBlocks;
-  } else if (kind != kMany && blocks > kOnePart) {
-    const int64_t want = (blocks * walks + kFewParts - 1) / kFewParts;
-    per = (want + 3) / 4 * 4;
-    if (per < kFewBlocks) per = kFewBlocks;
+  if (kind == kMany) {
+    int64_t per = blocks;
+    if (blocks > kManyOnePart) {
+      const int64_t splits = (kManyParts + a.c.B * walks - 1) / (a.c.B * walks);
+      per = (blocks + splits - 1) / splits;
+      if (per < kManyBlocks) per = kManyBlocks;
+    }
+    p.per = (int)(per < blocks ? per : blocks);
+    p.splits = (int)((blocks + p.per - 1) / p.per);
+  } else {  // a part holds at least kFewParts-th of all blocks, so each item adds one to kFewParts / walks
+    const int64_t each = (blocks + kFewBlocks - 1) / kFewBlocks, more = kFewParts / walks;
+    p.splits = (int)(blocks <= kOnePart ? a.c.B : a.c.B * each < a.c.B + more ? a.c.B * each : a.c.B + more);
   }
-  p.per = (int)(per < blocks ? per : blocks);
-  p.splits = (int)((blocks + p.per - 1) / p.per);
   return p;
+}
+
+// The slots of parts in the workspace; 0: no part is joined.
+int64_t slots_of(const CacheAttn& a, const Parts& p) {
+  if (p.per > 0) return p.splits > 1 ? (int64_t)p.splits * a.c.B : 0;
+  return p.splits > a.c.B ? p.splits : 0;
 }
 
 template <typename T, int D>
 hipError_t launch(const CacheAttn& a, hipStream_t stream) {
   Parts p = plan(a);
   const Kind kind = kind_of(a);
-  const int64_t heads = (int64_t)a.c.B * a.c.H, total = heads * a.group * a.S;
+  const int64_t heads = (int64_t)a.c.B * a.c.H, total = heads * a.group * a.S, slots = slots_of(a, p);
+  const int wide = wide_of(kind);
   p.o = reinterpret_cast<float*>(a.workspace);
-  p.ml = p.o + heads * p.tiles * p.splits * 16 * D;
-  const int wide = kind == kMany ? 128 : kind == kFew32 ? 32 : 16;
-  const int64_t walks = heads * p.splits, each = p.tiles / (wide / 16);  // few rows: in whole rounds of the XCDs
-  const dim3 grid((uint32_t)((kind == kMany ? walks : (walks + kNumXcd - 1) / kNumXcd * kNumXcd) * each)), threads(256);
+  p.ml = p.o + slots * a.c.H * p.tiles * 16 * D;
+  if (slots > 0) p.items = reinterpret_cast<int32_t*>(p.ml + slots * a.c.H * p.tiles * 32);
+  const int64_t each = p.tiles / (wide / 16);
+  const int64_t few = ((int64_t)p.splits * a.c.H + kNumXcd - 1) / kNumXcd * kNumXcd;  // in whole rounds of the XCDs
+  const dim3 grid((uint32_t)((kind == kMany ? heads * p.splits : few) * each)), threads(256);
   if (kind == kMany)
     hipLaunchKernelGGL((many_rows_kernel<T, D>), grid, threads, 0, stream, a, p);
   else if (kind == kFew32)
     hipLaunchKernelGGL((few_rows_kernel<T, D, 2>), grid, threads, 0, stream, a, p);
   else
     hipLaunchKernelGGL((few_rows_kernel<T, D, 1>), grid, threads, 0, stream, a, p);
-  if (p.splits > 1) {
+  if (slots > 0) {
     if (total <= kJoinRows)
       hipLaunchKernelGGL((join_kernel<T, D, 64>), dim3((uint32_t)((total + 3) / 4)), threads, 0, stream, a, p, wide, total);
     else
@@ -832,7 +866,8 @@ hipError_t launch(const CacheAttn& a, hipStream_t stream) {
 
 size_t cache_attn_workspace(const CacheAttn& a, int D) {
   const Parts p = plan(a);
-  return p.splits > 1 ? (size_t)a.c.B * a.c.H * p.tiles * p.splits * 16 * (D + 2) * sizeof(float) : 0;
+  const size_t slots = (size_t)slots_of(a, p);
+  return slots > 0 ? slots * a.c.H * p.tiles * 16 * (D + 2) * sizeof(float) + (size_t)a.c.B * 2 * sizeof(int32_t) : 0;
 }
 
 hipError_t launch_cache_attn(const CacheAttn& a, int dtype, int D, hipStream_t stream) {
