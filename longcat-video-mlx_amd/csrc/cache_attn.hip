@@ -8,13 +8,16 @@
 //   P' = exp2(u + ev - m),  m the running maximum of u + ev,
 //   O  = sum P' v8,         l = sum 2^-ev P',
 // so P' <= 1 in any mix of scales, O holds the true sum over 2^m, and l the softmax's
-// own denominator.  P' is rounded to T once (bf16 2^-9, fp16 2^-12 relative; an fp16
-// P' below 2^-14 loses bits only where the block with the larger values has an e4m3
-// step 2^16 times what is lost); sums, maxima and O stay in fp32.
+// own denominator.  P' is rounded to T once, after its sum (bf16 2^-9, fp16 2^-12 relative;
+// an fp16 P' below 2^-14 loses bits only where the block with the larger values has an e4m3
+// step 2^16 times what is lost); sums, maxima and O stay in fp32.  A P' below 2^-126 is
+// zero: where value scales 2^x apart meet, each token that l then lacks has a weight below
+// 2^(x - 126); fp16's range, zeros beside it, has x = 68.
 //
 // The rows of one key head are its group's queries, row r = query r / group of the
-// group's head r % group; a row sees the first `vis` tokens, rows in order no fewer.  What a row does not see has P' = 0, and
-// a NaN among the values of such tokens is taken out of its product.
+// group's head r % group; a row sees the first `vis` tokens, rows in order no fewer.  What
+// a row does not see has P' = 0, and a NaN among the values of such tokens is taken out of
+// its product.  A row all of whose scores are -inf counts as one that sees nothing.
 #include "cache_attn.h"
 
 namespace lcv {
@@ -57,7 +60,12 @@ __device__ __forceinline__ int64_t part_at(const CacheAttn& a, const Parts& p, i
 __device__ __forceinline__ int item_blocks(const CacheAttn& a, int b) { return (item_lens(a, b).len + 63) / 64; }
 
 // Few rows: the blocks of a part, so that all items together, `walks` times each, make
-// about kFewParts parts.  Wave-uniform.
+// about kFewParts parts, from the lengths, not from the bound on them: 4 requests of 3000
+// tokens in a cache of 65,536 take 12.5 us against 19.5 (6 tokens over 8200, 4097, 1 and
+// 12,000 22.2 against 21.6).  us: kFewParts 512 (640, 768): 8 requests over 168,716 tokens
+// 68 (75, 76), 32 heads over 18,720 33 (37, 37).  kFewBlocks 8 (4, 16): one token over 30,000
+// of one head 16 (21, 16), four over 2048 of 8 heads 15 (14, 17).  A walk of up to kOnePart
+// blocks is not worth a second launch: 24 rows over 1000 tokens 14.0, in parts of 8 18.3.
 constexpr int kFewParts = 512, kFewBlocks = 8, kOnePart = 16;
 __device__ __forceinline__ int few_per(const CacheAttn& a, int walks, int blocks) {  // blocks: item `lane`'s
   for (int b = 64 + threadIdx.x % 64; b < a.c.B; b += 64) blocks += item_blocks(a, b);
@@ -94,6 +102,12 @@ __device__ __forceinline__ int64_t lse_at(const CacheAttn& a, int b, int kvh, in
 // accumulators hold keys 16 G + 4 t + i of row gi, which is the order of the 16 bytes
 // that a lane reads of v8's row 16 dt + gi.  Keys and values of a wave's next block are
 // asked for as soon as those of this one are used.
+//
+// Bound by the cache's bytes: a token each of 8 requests over 168,716 tokens in all, 8 heads
+// of 128 (345 MB), takes 68 us with the join's 5, 5.1 TB/s (a copy of 1 GiB: 5.0); one over
+// 501 tokens 5.3 us, its loads' latency.  The next block's operands need the registers of
+// three waves a SIMD for 16 rows (74 us; two 79, four 111) and of two for 32 (24 rows of 8
+// heads over 9000 tokens 17 us; three 27).
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 1 ? 3 : 2, NT == 1 ? 3 : 2)))
 void few_rows_kernel(CacheAttn a, Parts p) {
@@ -332,7 +346,7 @@ void few_rows_kernel(CacheAttn a, Parts p) {
 
 // A row's parts together.  `wide` rows share a walk, whose reach says how many parts there
 // are.  THREADS threads take a row: a wave where there are few rows, so that many loads
-// are under way, 16 where there are many.
+// are under way, 16 where there are many (kJoinRows).
 template <typename T, int D, int THREADS>
 __global__ __launch_bounds__(256) void join_kernel(CacheAttn a, Parts p, int wide, int64_t total) {
   constexpr int kN = D / THREADS;
@@ -381,6 +395,9 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttn a, Parts p, int wid
   if (a.lse && lane == 0) a.lse[lse_at(a, b, kvh, r)] = empty ? kNegInf : (top + __builtin_log2f(lsum)) * kLn2;
 }
 
+// us: four prompts of 1 to 2048 queries over 391 to 5000 tokens 176 sorted, 233 in turn; four
+// items of 700 to 4000 tokens 157 and 218; eight equal ones of 512 tokens 22.5 and 21.4;
+// sixteen 27 and 23, as the search goes over the items.
 constexpr int kSorted = 8;
 
 // Which tile of 128 rows of which item a workgroup takes: the r-th of a key head's.
@@ -401,7 +418,9 @@ __device__ __forceinline__ Turn in_turn(const CacheAttn& a, int tiles, int r) {
 __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) {
   const int lane = threadIdx.x % 64;
   const Lens mine = item_lens(a, lane < a.c.B ? lane : 0);
-  auto item = [&](int b) { return Lens{__builtin_amdgcn_readlane(mine.len, b), __builtin_amdgcn_readlane(mine.ql, b)}; };
+  auto item = [&](int b) {
+    return Lens{__builtin_amdgcn_readlane(mine.len, b), __builtin_amdgcn_readlane(mine.ql, b)};
+  };
   auto real = [&](const Lens& n) { return (n.ql * a.group + 127) / 128; };  // tiles with queries
   auto reaching = [&](const Lens& n, int x) {  // how many of the item's tiles walk x blocks or more
     if (x == 0) return tiles;
@@ -444,7 +463,14 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 // A row's offset m is the maximum of its first half block, and later halves need no
 // maximum; their P' may pass 1.  Where a half's sum passes a bound (2^15 in fp16, whose
 // range ends there; 2^40 in bf16), or is NaN, the workgroup walks again with the rows'
-// exact maxima.  (Rescaling O inside the walk costs it 60 registers.)
+// exact maxima.  (Rescaling O inside the walk costs it 60 registers: 4310 us, below 3600.)
+//
+// Bound by instructions: a block costs a wave 64 MFMAs (1024 cycles), 32 exponentials with
+// their sums and 128 conversions of bytes, about 2350 cycles with the MFMAs beside them.
+// 12,480 queries of 32 heads of 128 over 18,720 tokens take 3.6 ms, 1062 TFLOP/s in bf16,
+// where a product of 8192^3 makes 1214.  D = 128 leaves registers for three waves a SIMD
+// (two: 3804 us, three 3580 then), D = 64 for four (4000 queries of 16 heads over 9000
+// tokens 195 us, three 200).
 template <typename T>
 constexpr float kMaxSum = 0x1p40f;
 template <>
@@ -473,7 +499,8 @@ void many_rows_kernel(CacheAttn a, Parts p) {
   const int tiles = p.tiles / 8;  // of 128 rows
   const int of_head = wid % (a.c.B * tiles), split = wid / (a.c.B * tiles) % p.splits;
   const int kvh = wid / (a.c.B * tiles * p.splits);
-  const Turn turn = a.c.B > 1 && a.c.B <= kSorted && p.splits == 1 ? by_length(a, tiles, of_head) : in_turn(a, tiles, of_head);
+  const bool sorted = a.c.B > 1 && a.c.B <= kSorted && p.splits == 1;
+  const Turn turn = sorted ? by_length(a, tiles, of_head) : in_turn(a, tiles, of_head);
   const int b = turn.b, tile = turn.tile;
   const int bh = b * a.c.H + kvh;
   const int tid = threadIdx.x, lane = tid % 64, G = lane / 16, gi = lane % 16;
@@ -791,8 +818,9 @@ void many_rows_kernel(CacheAttn a, Parts p) {
 }
 
 // Tiles of 32 rows straight from memory up to here, of 128 through LDS above.  us, 8 heads
-// over 1000 (9000) tokens, bf16, D = 128: 24 rows 18 (22) against 24 (26), 64 rows 18 (23)
-// against 25 (27), 96 rows 18 (25) against 25 (30), 128 rows 18 (31) against 26 (31).
+// over two items of 1000 (one of 9000, two of 40,000) tokens, bf16, D = 128: 64 rows 14 (23,
+// 56) against 19 (25, 69), 96 rows 14 (25, 69) against 20 (26, 71), 128 rows 14 (31, 80)
+// against 21 (29, 74).
 constexpr int kFewRows = 96;
 enum Kind { kFew16, kFew32, kMany };
 
@@ -801,7 +829,14 @@ Kind kind_of(const CacheAttn& a) {
   return rows <= 16 ? kFew16 : rows <= kFewRows ? kFew32 : kMany;
 }
 
+// Many rows: parts are written and joined in fp32, 64 KB a tile, so walks are split only
+// where there are fewer than two a CU.  us, D = 128, bf16: 512 walks of 32 blocks 78, in two
+// parts each 96, in five 122; D = 64, 500 walks of 141 blocks 198 in two, 222 in one.  Parts
+// of at least kManyBlocks 6 (4, 8): 128 rows of 8 heads over 9000 tokens 28 (28, 30), over
+// two items of 1000 20 (20, 24), 2048 causal queries of 4 heads over one key head 30 (31,
+// 29).  128 walks of up to kManyOnePart 8 blocks 20.5, in two parts 23.5.
 constexpr int64_t kManyParts = 512, kManyBlocks = 6, kManyOnePart = 8;
+// us, walk and join: 256 rows 73 with a wave a row, 78 with 16 threads; 64,000 rows 212, 192.
 constexpr int64_t kJoinRows = 4096;
 
 int wide_of(Kind kind) { return kind == kMany ? 128 : kind == kFew32 ? 32 : 16; }
