@@ -211,9 +211,13 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
     ``q_lens``: how many of the S queries of each item are real (default: all).
     ``causal``: the real queries are the item's last tokens, and query i sees the
     tokens up to ``lengths - q_lens + i``.  Rows that see nothing (padding, empty
-    items, queries before the first token) get zeros.  ``max_len``: a bound on
-    ``lengths`` known to the caller (longer items count as that long); it shapes the
-    launch, so a close one serves short histories in a long cache.
+    items, queries before the first token) get zeros, as do rows all of whose scores
+    are -inf.  ``max_len``: a bound on ``lengths`` known to the caller (longer items
+    count as that long); it shapes the launch of many rows, so a close one serves
+    short histories in a long cache.
+
+    Sums are fp32.  Where the scales of the values that a row sees are 2^x apart, a
+    token whose weight is below 2^(x - 126) may be left out of the row's sum.
 
     Returns ``out`` ``[B, Hq, S, D]`` in q's dtype, or ``(out, lse)`` with the fp32
     ``[B, Hq, S]`` log of each row's sum (-inf where nothing is seen)."""

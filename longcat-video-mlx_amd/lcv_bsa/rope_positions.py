@@ -124,7 +124,10 @@ def rope_nd(x: torch.Tensor, positions: torch.Tensor, dims: Optional[Sequence[in
 
     ``dims``: the even number of dims that each axis turns, summing to D; by
     default the t / h / w split of ``rope_dims`` for three axes, else equal
-    parts.  Differentiable in ``x`` (as often as wanted); positions get no gradient."""
+    parts.  Differentiable in ``x`` (as often as wanted); positions get no gradient.
+    A backward pass that is captured into a graph takes its gradients with
+    ``torch.autograd.grad``, while no graph of the same leaves that was made outside
+    of the capture is alive: torch would have to order the two streams there."""
     _require_device(x, positions)
     if x.dim() != 4:
         raise ValueError(f"x must be [B, H, S, D], got shape {tuple(x.shape)}")
