@@ -462,7 +462,8 @@ int lcv_bsa_prepare_qkv(const void* q_in, const void* k_in, const void* v_in,
  *   out[2p] = x[2p] cos theta - x[2p+1] sin theta,
  *   out[2p+1] = x[2p] sin theta + x[2p+1] cos theta,
  * and with -theta where `inverse` is set: the gradient.  x, out [B,H,S,D], D % 8
- * == 0, D <= 256, rows on 16-byte boundaries; out may be x itself.  positions
+ * == 0, D <= 256, rows on 16-byte boundaries; out may be x itself, with x's
+ * strides, and does not overlap it otherwise.  positions
  * [B or 1, S, axes] of type int32 (0), int64 (1) or fp32 (2), the axes next to one
  * another, strides in elements (batch stride 0: shared).  dims (host memory) holds
  * the axes' dims: even, summing to D.  Angles are taken in 64 bits.
@@ -529,7 +530,7 @@ int lcv_bsa_cached_attn(const void* q, int dtype, int64_t Hq, int64_t S,
  * What each cached token got from these queries: out[b,h,j] = weights[b,h,j] +
  * the sum over the queries of key head h that see token j of exp(sm_scale q.k_j -
  * lse), with lse from lcv_bsa_cached_attn.  weights (null: zeros) and out are
- * [B,H,capacity] fp32, and may be one.  The sums' order is fixed.  The workspace
+ * [B,H,capacity] fp32, one buffer or two apart.  The sums' order is fixed.  The workspace
  * holds the sums of parts of the rows.
  */
 size_t lcv_bsa_attention_weights_workspace_bytes(int64_t Hq, int64_t S,

@@ -1093,6 +1093,8 @@ int lcv_bsa_rope_nd(const void* x, int dtype, int64_t B, int64_t H, int64_t S, i
   const int vec = 16 / elem_bytes(dtype);
   if (!vec_aligned(x, xs, vec) || !vec_aligned(out, os, vec))
     return fail(LCV_BSA_ERR_LAYOUT, "x and out rows must start on 16-byte boundaries");
+  if (x == out && (xs.b != os.b || xs.h != os.h || xs.s != os.s))
+    return fail(LCV_BSA_ERR_LAYOUT, "in place, x and out must have the same strides");
   lcv::RopeNd r{};
   int64_t pair = 0;
   for (int64_t a = 0; a < axes; ++a) {
@@ -1172,6 +1174,10 @@ int lcv_bsa_attention_weights(const void* q, int dtype, int64_t Hq, int64_t S, l
   const int st = check_cache_attn(q, dtype, Hq, S, qs, c, lengths, q_lens, causal, sm_scale, max_len, &a);
   if (st) return st;
   if (!lse || !out) return fail(LCV_BSA_ERR_INVALID_ARG, "null pointer");
+  const uintptr_t from = (uintptr_t)weights, to = (uintptr_t)out;
+  const uintptr_t bytes = (uintptr_t)c.B * (uintptr_t)c.H * (uintptr_t)c.capacity * sizeof(float);
+  if (weights && from != to && (from < to ? to - from : from - to) < bytes)
+    return fail(LCV_BSA_ERR_INVALID_ARG, "weights and out overlap in part");
   if (qs.s >= (int64_t)1 << 25)  // 32 rows are addressed in 32 bits
     return fail(LCV_BSA_ERR_LAYOUT, "q's rows are 2^25 elements or more apart");
   a.lse = const_cast<float*>(lse);

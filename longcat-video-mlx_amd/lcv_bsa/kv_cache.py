@@ -44,7 +44,7 @@ class KVCache8:
     two in [2^-60, 2^60].  Contiguous, D 64 or 128.  How many tokens of it are in
     use is its user's to say, at every call."""
 
-    __slots__ = ("k8", "v8", "k_scale", "v_scale", "_c")
+    __slots__ = ("_tensors", "_c")
 
     def __init__(self, k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         _require_device(k8, v8, k_scale, v_scale)
@@ -67,7 +67,7 @@ class KVCache8:
         if ((kp | vp) % 16 or not k8.is_contiguous() or not v8.is_contiguous() or not k_scale.is_contiguous()
                 or not v_scale.is_contiguous()):
             raise ValueError("a cache's tensors must be contiguous, k8 and v8 on 16-byte boundaries")
-        self.k8, self.v8, self.k_scale, self.v_scale = k8, v8, k_scale, v_scale
+        self._tensors = k8, v8, k_scale, v_scale
         self._c = _lib.Cache8(kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), B, H, n, D)
 
     @classmethod
@@ -79,6 +79,28 @@ class KVCache8:
                    torch.zeros((batch, heads, nb, head_dim, BLOCK), dtype=torch.uint8, device=dev).view(_E4M3),
                    torch.ones((batch, heads, nb), dtype=torch.float32, device=dev),
                    torch.ones((batch, heads, nb), dtype=torch.float32, device=dev))
+
+    @property
+    def k8(self) -> torch.Tensor:
+        return self._tensors[0]
+
+    @property
+    def v8(self) -> torch.Tensor:
+        return self._tensors[1]
+
+    @property
+    def k_scale(self) -> torch.Tensor:
+        return self._tensors[2]
+
+    @property
+    def v_scale(self) -> torch.Tensor:
+        return self._tensors[3]
+
+    def _pointers(self) -> _lib.Cache8:
+        """The cache as the entry points read it: where its tensors lie now."""
+        c, (k8, v8, k_scale, v_scale) = self._c, self._tensors
+        c.k8, c.v8, c.k_scale, c.v_scale = k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
+        return c
 
     @property
     def shape(self) -> tuple[int, int, int, int]:
@@ -169,8 +191,8 @@ def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start: Ints,
     k, ks = rows_of(k, "k")
     v, vs = rows_of(v, "v")
     with on_device(k):
-        st = _lib.load().lcv_bsa_cache_append(cache._c, k.data_ptr(), v.data_ptr(), code, S, ks, vs, start.data_ptr(),
-                                              None if counts is None else counts.data_ptr(), _stream(k))
+        st = _lib.load().lcv_bsa_cache_append(cache._pointers(), k.data_ptr(), v.data_ptr(), code, S, ks, vs,
+                                              start.data_ptr(), None if counts is None else counts.data_ptr(), _stream(k))
     _lib.check(st, "cache_append")
     return cache
 
@@ -244,7 +266,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
     size = _workspace("lcv_bsa_cached_attn_workspace_bytes", Hq, S, *cache.shape, max_len)
     ws = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
     with on_device(q):
-        st = lib.lcv_bsa_cached_attn(q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._c, lengths.data_ptr(),
+        st = lib.lcv_bsa_cached_attn(q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._pointers(), lengths.data_ptr(),
                                      None if q_lens is None else q_lens.data_ptr(), int(causal), sm_scale, max_len,
                                      to.data_ptr(), os, None if lse is None else lse.data_ptr(),
                                      None if ws is None else ws.data_ptr(), size, _stream(q))
@@ -289,7 +311,7 @@ def attention_weights(q: torch.Tensor, cache: KVCache8, lengths: Ints, lse: torc
     ws = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
     with on_device(q):
         st = lib.lcv_bsa_attention_weights(
-            q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._c, lengths.data_ptr(),
+            q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._pointers(), lengths.data_ptr(),
             None if q_lens is None else q_lens.data_ptr(), int(causal), sm_scale, max_len, lse.data_ptr(),
             None if weights is None else weights.data_ptr(), out.data_ptr(), None if ws is None else ws.data_ptr(), size,
             _stream(q))
@@ -325,7 +347,8 @@ def cache_evict(cache: KVCache8, lengths: Ints, weights: torch.Tensor, keep: int
     kept = torch.empty((B, H, keep), dtype=torch.int32, device=dev)
     left = torch.empty((B,), dtype=torch.int32, device=dev)
     with on_device(weights):
-        st = _lib.load().lcv_bsa_cache_evict(cache._c, lengths.data_ptr(), weights.data_ptr(), keep, recent, new._c,
-                                             new_weights.data_ptr(), kept.data_ptr(), left.data_ptr(), _stream(weights))
+        st = _lib.load().lcv_bsa_cache_evict(cache._pointers(), lengths.data_ptr(), weights.data_ptr(), keep, recent,
+                                             new._pointers(), new_weights.data_ptr(), kept.data_ptr(), left.data_ptr(),
+                                             _stream(weights))
     _lib.check(st, "cache_evict")
     return new, new_weights, kept, left

@@ -238,3 +238,32 @@ def test_reference_attention_is_softmax():
     want = torch.softmax(t, -1).nan_to_num(0.0) @ v
     torch.testing.assert_close(out, want)
     torch.testing.assert_close(lse, torch.logsumexp(t, -1))
+
+
+def test_a_cache_keeps_its_tensors(on_cpu):
+    """They cannot be exchanged for others, and what is passed on is where they are."""
+    c = _cache()
+    for name in ("k8", "v8", "k_scale", "v_scale"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name).clone())
+    moved = c.k_scale.clone()
+    c.k_scale.data = moved
+    p = c._pointers()
+    assert (p.k8, p.v8, p.k_scale, p.v_scale) == (c.k8.data_ptr(), c.v8.data_ptr(), moved.data_ptr(), c.v_scale.data_ptr())
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="validation-only calls use fake pointers; CPU container only")
+def test_c_entries_refuse_overlaps():
+    import ctypes
+
+    from lcv_bsa import _lib
+
+    lib, fake = _lib.load(), 1 << 20
+    st = _lib.Strides(8192, 4096, 64)
+    c = _lib.Cache8(k8=fake, v8=fake, k_scale=fake, v_scale=fake, B=1, H=2, capacity=128, D=64)
+    for apart in (4, 1020, -4, -1020):  # of 1024 bytes
+        assert lib.lcv_bsa_attention_weights(fake, 1, 2, 4, st, c, fake, None, 0, 0.1, 64, fake, fake, fake + apart, None, 0, None) == _lib.ERR_INVALID_ARG
+        assert b"overlap" in lib.lcv_bsa_last_error()
+    other = _lib.Strides(8192, 64, 128)
+    assert lib.lcv_bsa_rope_nd(fake, 1, 1, 2, 4, 64, st, fake, 0, 0, 1, (ctypes.c_int64 * 1)(64), 1, 1e4, 0, fake, other, None) == _lib.ERR_LAYOUT
+    assert b"in place" in lib.lcv_bsa_last_error()

@@ -308,3 +308,31 @@ def test_rotary_rows_beyond_32_bits(device):
     assert torch.equal(rope_nd(x, pos)[:, -2:], want)
     turned = x.transpose(1, 2).contiguous().transpose(1, 2)
     assert torch.equal(rope_nd(turned, pos)[:, -2:], want)
+
+
+@pytest.mark.parametrize("S", [1, 6, 40, 150])
+def test_out_may_be_q(device, S):
+    """A row is read before it is written, and by its own workgroups alone."""
+    from lcv_bsa import cached_attention
+
+    gen = _gen(device, S)
+    c = _cache(gen, device, 2, 2, 2048, 64)
+    n = _ints(device, [2000, 130])
+    q = torch.randn(2, 8, S, 64, generator=gen, device=device).to(BF16)
+    want = cached_attention(q, c, n, causal=True)
+    assert cached_attention(q, c, n, causal=True, out=q) is q and torch.equal(q, want)
+
+
+def test_moved_tensors(device):
+    """A cache whose tensors were given other memory is read where they are."""
+    from lcv_bsa import cached_attention
+
+    gen = _gen(device, 1)
+    c = _cache(gen, device, 1, 2, 128, 64)
+    q = torch.randn(1, 2, 3, 64, generator=gen, device=device).to(F16)
+    want = cached_attention(q, c, 100)
+    for t in (c.k8, c.v8, c.k_scale, c.v_scale):
+        old = t.detach()  # the memory that it leaves
+        t.data = old.view(torch.uint8).clone().view(t.dtype)
+        old.view(torch.uint8).zero_()
+    assert torch.equal(cached_attention(q, c, 100), want)
