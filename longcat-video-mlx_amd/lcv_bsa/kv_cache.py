@@ -26,8 +26,8 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .block_sparse_attention import _dtype_code, _require_device, _stream
-from .rope_positions import on_device, rows_of
+from .block_sparse_attention import _dtype_code, _require_device
+from .rope_positions import launch, rows_of
 
 __all__ = ["KVCache8", "cache_append", "cached_attention", "attention_weights", "cache_evict"]
 
@@ -44,7 +44,7 @@ class KVCache8:
     two in [2^-60, 2^60].  Contiguous, D 64 or 128.  How many tokens of it are in
     use is its user's to say, at every call."""
 
-    __slots__ = ("_tensors", "_c")
+    __slots__ = ("_tensors", "_shape")
 
     def __init__(self, k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         _require_device(k8, v8, k_scale, v_scale)
@@ -63,12 +63,11 @@ class KVCache8:
                 or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32):
             raise ValueError(f"k_scale and v_scale must be fp32 {(B, H, nb)}, got {k_scale.dtype} {tuple(k_scale.shape)} "
                              f"and {v_scale.dtype} {tuple(v_scale.shape)}")
-        kp, vp = k8.data_ptr(), v8.data_ptr()
-        if ((kp | vp) % 16 or not k8.is_contiguous() or not v8.is_contiguous() or not k_scale.is_contiguous()
-                or not v_scale.is_contiguous()):
+        if ((k8.data_ptr() | v8.data_ptr()) % 16 or not k8.is_contiguous() or not v8.is_contiguous()
+                or not k_scale.is_contiguous() or not v_scale.is_contiguous()):
             raise ValueError("a cache's tensors must be contiguous, k8 and v8 on 16-byte boundaries")
         self._tensors = k8, v8, k_scale, v_scale
-        self._c = _lib.Cache8(kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), B, H, n, D)
+        self._shape = B, H, n, D
 
     @classmethod
     def empty(cls, batch: int, heads: int, capacity: int, head_dim: int, device=None) -> "KVCache8":
@@ -98,19 +97,17 @@ class KVCache8:
 
     def _pointers(self) -> _lib.Cache8:
         """The cache as the entry points read it: where its tensors lie now."""
-        c, (k8, v8, k_scale, v_scale) = self._c, self._tensors
-        c.k8, c.v8, c.k_scale, c.v_scale = k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
-        return c
+        k8, v8, k_scale, v_scale = self._tensors
+        return _lib.Cache8(k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *self._shape)
 
     @property
     def shape(self) -> tuple[int, int, int, int]:
         """(batch, heads, capacity, head_dim)."""
-        c = self._c
-        return c.B, c.H, c.capacity, c.D
+        return self._shape
 
     @property
     def capacity(self) -> int:
-        return self.k8.shape[2]
+        return self._shape[2]
 
     @property
     def device(self) -> torch.device:
@@ -190,10 +187,8 @@ def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start: Ints,
         return cache
     k, ks = rows_of(k, "k")
     v, vs = rows_of(v, "v")
-    with on_device(k):
-        st = _lib.load().lcv_bsa_cache_append(cache._pointers(), k.data_ptr(), v.data_ptr(), code, S, ks, vs,
-                                              start.data_ptr(), None if counts is None else counts.data_ptr(), _stream(k))
-    _lib.check(st, "cache_append")
+    launch(k, "cache_append", cache._pointers(), k.data_ptr(), v.data_ptr(), code, S, ks, vs, start.data_ptr(),
+           None if counts is None else counts.data_ptr())
     return cache
 
 
@@ -262,15 +257,11 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
         return (out, lse) if return_lse else out
     q, qs = rows_of(q, "q")
     to, os = rows_of(out, "out")  # a copy where out's rows cannot be written in place
-    lib = _lib.load()
     size = _workspace("lcv_bsa_cached_attn_workspace_bytes", Hq, S, *cache.shape, max_len)
     ws = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
-    with on_device(q):
-        st = lib.lcv_bsa_cached_attn(q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._pointers(), lengths.data_ptr(),
-                                     None if q_lens is None else q_lens.data_ptr(), int(causal), sm_scale, max_len,
-                                     to.data_ptr(), os, None if lse is None else lse.data_ptr(),
-                                     None if ws is None else ws.data_ptr(), size, _stream(q))
-    _lib.check(st, "cached_attention")
+    launch(q, "cached_attn", q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._pointers(), lengths.data_ptr(),
+           None if q_lens is None else q_lens.data_ptr(), int(causal), sm_scale, max_len, to.data_ptr(), os,
+           None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), size)
     if to is not out:
         out.copy_(to)
     return (out, lse) if return_lse else out
@@ -306,16 +297,11 @@ def attention_weights(q: torch.Tensor, cache: KVCache8, lengths: Ints, lse: torc
     q, qs = rows_of(q, "q")
     lse = lse.contiguous()
     weights = None if weights is None else weights.contiguous()
-    lib = _lib.load()
     size = _workspace("lcv_bsa_attention_weights_workspace_bytes", Hq, S, *cache.shape, max_len)
     ws = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
-    with on_device(q):
-        st = lib.lcv_bsa_attention_weights(
-            q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._pointers(), lengths.data_ptr(),
-            None if q_lens is None else q_lens.data_ptr(), int(causal), sm_scale, max_len, lse.data_ptr(),
-            None if weights is None else weights.data_ptr(), out.data_ptr(), None if ws is None else ws.data_ptr(), size,
-            _stream(q))
-    _lib.check(st, "attention_weights")
+    launch(q, "attention_weights", q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._pointers(), lengths.data_ptr(),
+           None if q_lens is None else q_lens.data_ptr(), int(causal), sm_scale, max_len, lse.data_ptr(),
+           None if weights is None else weights.data_ptr(), out.data_ptr(), None if ws is None else ws.data_ptr(), size)
     return out
 
 
@@ -346,9 +332,6 @@ def cache_evict(cache: KVCache8, lengths: Ints, weights: torch.Tensor, keep: int
     new_weights = torch.empty((B, H, nb * BLOCK), dtype=torch.float32, device=dev)
     kept = torch.empty((B, H, keep), dtype=torch.int32, device=dev)
     left = torch.empty((B,), dtype=torch.int32, device=dev)
-    with on_device(weights):
-        st = _lib.load().lcv_bsa_cache_evict(cache._pointers(), lengths.data_ptr(), weights.data_ptr(), keep, recent,
-                                             new._pointers(), new_weights.data_ptr(), kept.data_ptr(), left.data_ptr(),
-                                             _stream(weights))
-    _lib.check(st, "cache_evict")
+    launch(weights, "cache_evict", cache._pointers(), lengths.data_ptr(), weights.data_ptr(), keep, recent,
+           new._pointers(), new_weights.data_ptr(), kept.data_ptr(), left.data_ptr())
     return new, new_weights, kept, left

@@ -26,38 +26,42 @@ __all__ = ["rope_nd", "grid_positions"]
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
-class on_device:
-    """Makes ``t``'s device the current one for a launch (nothing where it is)."""
+def launch(t: torch.Tensor, name: str, *args) -> None:
+    """The entry point ``lcv_bsa_<name>`` with ``t``'s device current, on that device's
+    current stream (its last argument)."""
+    entry = getattr(_lib.load(), "lcv_bsa_" + name)
+    index = t.device.index
+    if torch._C._cuda_getDevice() == index:
+        status = entry(*args, _stream(t))
+    else:
+        with torch.cuda.device(index):
+            status = entry(*args, _stream(t))
+    if status:
+        _lib.check(status, name)
 
-    __slots__ = ("index", "before")
 
-    def __init__(self, t: torch.Tensor):
-        self.index = t.device.index
-
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        self.before = None if now == self.index else now
-        if self.before is not None:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
+@functools.lru_cache(maxsize=4096)
+def _row_strides(shape: tuple, strides: tuple, size: int) -> Optional[_lib.Strides]:
+    """The strides of [B, H, S, D] as the kernels read it (those of dimensions of size one
+    put right); None where its rows are not dense, overlap or leave 16-byte boundaries."""
+    (B, H, S, D), (sb, sh, ss, sd) = shape, strides
+    sb, sh, ss = sb if B > 1 else D, sh if H > 1 else D, ss if S > 1 else D
+    if (sd != 1 and D > 1) or ss < D or (sb | sh | ss) * size % 16:
+        return None
+    return _lib.Strides(sb, sh, ss)
 
 
 def rows_of(t: torch.Tensor, name: str) -> tuple[torch.Tensor, _lib.Strides]:
     """``t`` [B, H, S, D] as the kernels read it -- rows dense, on 16-byte
-    boundaries, not overlapping -- copied where it is not, and its strides (those
-    of dimensions of size one put right)."""
+    boundaries, not overlapping -- copied where it is not, and its strides."""
     if t.dim() != 4:
         raise ValueError(f"{name} must be [B, H, S, D], got shape {tuple(t.shape)}")
-    B, H, S, D = t.shape
-    sb, sh, ss, sd = t.stride()
-    sb, sh, ss = sb if B > 1 else D, sh if H > 1 else D, ss if S > 1 else D
-    if (sd != 1 and D > 1) or ss < D or (sb | sh | ss) * t.element_size() % 16 or t.data_ptr() % 16:
+    strides = _row_strides(t.shape, t.stride(), t.element_size())
+    if strides is None or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-        return t, _lib.Strides(H * S * D, S * D, D)
-    return t, _lib.Strides(sb, sh, ss)
+        _, H, S, D = t.shape
+        strides = _lib.Strides(H * S * D, S * D, D)
+    return t, strides
 
 
 def grid_positions(grid: Sequence[int], first: Sequence[int] = (0, 0, 0), device=None) -> torch.Tensor:
@@ -67,7 +71,6 @@ def grid_positions(grid: Sequence[int], first: Sequence[int] = (0, 0, 0), device
     return torch.stack(torch.meshgrid(*axes, indexing="ij"), -1).reshape(-1, len(axes))
 
 
-@functools.lru_cache(maxsize=256)
 def _split(D: int, axes: int, dims: Optional[tuple]):
     """The axes' dims (checked; None: the default split) as the entry point reads them."""
     if D % 8 or not 8 <= D <= 256:
@@ -82,23 +85,45 @@ def _split(D: int, axes: int, dims: Optional[tuple]):
     return (ctypes.c_int64 * axes)(*dims)
 
 
-def _rotate(x: torch.Tensor, positions: torch.Tensor, dims, base: float, inverse: bool) -> torch.Tensor:
-    B, H, S, D = x.shape
-    out = torch.empty_like(x)
-    if not x.numel():
+@functools.lru_cache(maxsize=1024)
+def _plan(shape: tuple, strides: tuple, dtype: torch.dtype, pshape: tuple, pstrides: tuple, ptype: torch.dtype,
+          dims: Optional[tuple]):
+    """The checks of a rotation, and what follows from the sizes, strides and types alone:
+    (dtype code, position code, positions' strides or None for a copy of them, dims,
+    output's strides, whether the output lies in memory like x)."""
+    if len(shape) != 4:
+        raise ValueError(f"x must be [B, H, S, D], got shape {tuple(shape)}")
+    x = torch.empty_strided(shape, strides, dtype=dtype, device="meta")
+    code = _dtype_code(x)
+    B, H, S, D = shape
+    if len(pshape) not in (2, 3) or pshape[-2] != S or (len(pshape) == 3 and pshape[0] not in (1, B)):
+        raise ValueError(f"positions must be [{S}, axes] or [{B} or 1, {S}, axes], got {tuple(pshape)}")
+    if ptype not in _POSITION_TYPES:
+        raise ValueError(f"positions must be int32, int64 or float32, got {ptype}")
+    split = _split(D, pshape[-1], dims)
+    where = None
+    if pshape[-1] == 1 or pstrides[-1] == 1:
+        where = (pstrides[0] if len(pshape) == 3 and pshape[0] > 1 else 0, pstrides[-2])
+    like = torch.empty_like(x).stride()
+    alike = like[3] == 1 and like[2] >= D
+    os = _row_strides(shape, like if alike else (H * S * D, S * D, D, 1), x.element_size())
+    return code, _POSITION_TYPES[ptype], where, split, os, alike
+
+
+def _rotate(x: torch.Tensor, positions: torch.Tensor, dims: Optional[tuple], base: float, inverse: bool) -> torch.Tensor:
+    shape = x.shape
+    code, pcode, where, split, os, alike = _plan(shape, x.stride(), x.dtype, positions.shape, positions.stride(),
+                                                 positions.dtype, dims)
+    out = torch.empty_like(x) if alike else torch.empty(shape, dtype=x.dtype, device=x.device)
+    B, H, S, D = shape
+    if not B * H * S:
         return out
-    sb, sh, ss, sd = out.stride()
-    if sd != 1 or ss < D:  # x itself is not dense
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        sb, sh, ss, sd = out.stride()
+    if where is None:
+        positions = positions.contiguous()
+        where = positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0, positions.stride(-2)
     x, xs = rows_of(x, "x")
-    ps = positions.stride()
-    with on_device(x):
-        st = _lib.load().lcv_bsa_rope_nd(
-            x.data_ptr(), _dtype_code(x), B, H, S, D, xs, positions.data_ptr(), _POSITION_TYPES[positions.dtype],
-            ps[0] if len(ps) == 3 and positions.shape[0] > 1 else 0, ps[-2], dims, len(dims), base, inverse,
-            out.data_ptr(), _lib.Strides(sb if B > 1 else D, sh if H > 1 else D, ss if S > 1 else D), _stream(x))
-    _lib.check(st, "rope_nd")
+    launch(x, "rope_nd", x.data_ptr(), code, B, H, S, D, xs, positions.data_ptr(), pcode, *where, split, len(split), base,
+           inverse, out.data_ptr(), os)
     return out
 
 
@@ -129,20 +154,9 @@ def rope_nd(x: torch.Tensor, positions: torch.Tensor, dims: Optional[Sequence[in
     ``torch.autograd.grad``, while no graph of the same leaves that was made outside
     of the capture is alive: torch would have to order the two streams there."""
     _require_device(x, positions)
-    if x.dim() != 4:
-        raise ValueError(f"x must be [B, H, S, D], got shape {tuple(x.shape)}")
-    _dtype_code(x)
-    B, _, S, D = x.shape
-    if positions.dim() not in (2, 3) or positions.shape[-2] != S or (positions.dim() == 3 and positions.shape[0] not in (1, B)):
-        raise ValueError(f"positions must be [{S}, axes] or [{B} or 1, {S}, axes], got {tuple(positions.shape)}")
-    if positions.dtype not in _POSITION_TYPES:
-        raise ValueError(f"positions must be int32, int64 or float32, got {positions.dtype}")
-    split = _split(D, positions.shape[-1], None if dims is None else tuple(dims))
+    dims = None if dims is None else tuple(dims)
     if positions.requires_grad:
         positions = positions.detach()
-    ps = positions.stride()
-    if ps[-1] != 1 or min(ps) < 0:
-        positions = positions.contiguous()
     if x.requires_grad and torch.is_grad_enabled():
-        return _RopeNd.apply(x, positions, split, float(base), False)
-    return _rotate(x, positions, split, float(base), False)
+        return _RopeNd.apply(x, positions, dims, float(base), False)
+    return _rotate(x, positions, dims, float(base), False)

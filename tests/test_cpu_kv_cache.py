@@ -2,7 +2,6 @@
 
 from __future__ import annotations
 
-import contextlib
 import math
 
 import pytest
@@ -23,7 +22,6 @@ def on_cpu(monkeypatch):
 
     for m in (kv_cache, rope_positions):
         monkeypatch.setattr(m, "_require_device", lambda *ts: None)
-        monkeypatch.setattr(m, "on_device", lambda t: contextlib.nullcontext())
     monkeypatch.setattr(_lib, "load", no_launch)
 
 
