@@ -70,6 +70,13 @@ class KVCache8:
         self._shape = B, H, n, D
 
     @classmethod
+    def _of(cls, k8, v8, k_scale, v_scale) -> "KVCache8":
+        """A cache of new tensors, whose shapes need no checks."""
+        cache = object.__new__(cls)
+        cache._tensors, cache._shape = (k8, v8, k_scale, v_scale), tuple(k8.shape)
+        return cache
+
+    @classmethod
     def empty(cls, batch: int, heads: int, capacity: int, head_dim: int, device=None) -> "KVCache8":
         """A cache of zeros with room for ``capacity`` tokens (rounded up to a block)."""
         dev = torch.device("cuda") if device is None else torch.device(device)
@@ -130,7 +137,7 @@ class KVCache8:
             new = torch.empty((batch, H, nb, *shape), dtype=t.dtype, device=t.device)
             new[:, :, :old] = t
             parts.append(new)
-        return KVCache8(parts[0].view(_E4M3).view(batch, H, nb * BLOCK, D), parts[1].view(_E4M3), *parts[2:])
+        return self._of(parts[0].view(_E4M3).view(batch, H, nb * BLOCK, D), parts[1].view(_E4M3), *parts[2:])
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values ``[B, H, capacity, D]`` as numbers."""
@@ -241,7 +248,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
     lengths, q_lens, sm_scale, max_len = _queries("cached_attention", q, cache, lengths, q_lens, sm_scale, max_len)
     B, Hq, S, D = q.shape
     if out is None:
-        out = torch.empty((B, Hq, S, D), dtype=q.dtype, device=q.device)
+        out = q.new_empty((B, Hq, S, D))
     else:
         _require_device(q, out)
         _no_grad("cached_attention", out)
@@ -249,7 +256,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
             raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
         if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
             raise ValueError("out's elements share memory")
-    lse = torch.empty((B, Hq, S), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = cache.k_scale.new_empty((B, Hq, S)) if return_lse else None
     if q.numel() == 0 or max_len == 0:
         out.zero_()
         if return_lse:
@@ -287,7 +294,7 @@ def attention_weights(q: torch.Tensor, cache: KVCache8, lengths: Ints, lse: torc
     _require_device(q, lse, *(t for t in (weights, out) if t is not None))
     _no_grad("attention_weights", lse, *(t for t in (weights, out) if t is not None))
     if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=q.device)
+        out = lse.new_empty(shape)
     elif not out.is_contiguous():
         raise ValueError("out must be contiguous")
     if q.numel() == 0 or max_len == 0:
@@ -324,14 +331,9 @@ def cache_evict(cache: KVCache8, lengths: Ints, weights: torch.Tensor, keep: int
         raise ValueError(f"keep={keep} must be at least 1 and recent={recent} in [0, keep]")
     lengths = _ints(lengths, "lengths", B, cache.device, 0, n)
     weights = weights.contiguous()
-    dev, nb = cache.device, -(-keep // BLOCK)
-    new = KVCache8(torch.empty((B, H, nb * BLOCK, D), dtype=_E4M3, device=dev),
-                   torch.empty((B, H, nb, D, BLOCK), dtype=_E4M3, device=dev),
-                   torch.empty((B, H, nb), dtype=torch.float32, device=dev),
-                   torch.empty((B, H, nb), dtype=torch.float32, device=dev))
-    new_weights = torch.empty((B, H, nb * BLOCK), dtype=torch.float32, device=dev)
-    kept = torch.empty((B, H, keep), dtype=torch.int32, device=dev)
-    left = torch.empty((B,), dtype=torch.int32, device=dev)
+    nb, words, numbers = -(-keep // BLOCK), cache.k8.new_empty, weights.new_empty
+    new = KVCache8._of(words((B, H, nb * BLOCK, D)), words((B, H, nb, D, BLOCK)), numbers((B, H, nb)), numbers((B, H, nb)))
+    new_weights, kept, left = numbers((B, H, nb * BLOCK)), lengths.new_empty((B, H, keep)), lengths.new_empty((B,))
     launch(weights, "cache_evict", cache._pointers(), lengths.data_ptr(), weights.data_ptr(), keep, recent,
            new._pointers(), new_weights.data_ptr(), kept.data_ptr(), left.data_ptr())
     return new, new_weights, kept, left
