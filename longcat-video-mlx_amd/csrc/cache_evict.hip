@@ -15,7 +15,7 @@
 // whose bytes lie token by token, a wave takes one of the D rows at a time, its lanes the
 // 64 tokens: kept tokens are in order, so the lanes' bytes are in few lines.
 //
-// 9360 of 18,720 tokens of 32 heads of 128: ranking 19 us (32 workgroups, bound by the
+// 9360 of 18,720 tokens of 32 heads of 128: ranking 17 us (32 workgroups, bound by the
 // passes' latency), gathering 40 us: 192 MB, as of the values every line is read, 4.8 TB/s.
 #include "cache_common.h"
 
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(kRankThreads) void rank_kernel(const int32_t* lengt
   __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];  // later: the last candidates
   __shared__ uint32_t waves[2][kRankWaves];
   __shared__ uint32_t found[3];
-  __shared__ uint32_t held[N + 192];  // past the end: read four at a time
+  __shared__ __attribute__((aligned(16))) uint32_t held[N > 0 ? N : 4];
   const int bh = blockIdx.x, b = bh / H;
   const int tid = threadIdx.x, lane = tid % 64, wave = uniform_i32(tid / 64);
   int64_t n = lengths[b];
@@ -57,47 +57,42 @@ __global__ __launch_bounds__(kRankThreads) void rank_kernel(const int32_t* lengt
   const int want = left - tail;  // of them stay
   const float* w = weights + (int64_t)bh * capacity;
 
-  // Wave w holds tokens w * run .. + run - 1, its lane l tokens r * 64 + l of them.
-  const int per = (len + kRankThreads - 1) / kRankThreads, run = per * 64, first = wave * run + lane;
-  // Some weights at a time, so that their loads (from memory or LDS) are under way together;
-  // the compiler unrolls no loop over ballots.
-  auto keys = [&](int r0, auto& k) {
-    constexpr int n = sizeof(k) / 4;
-    float x[n];
+  // Wave w holds tokens w * run .. + run - 1, its lane l four of each 256.
+  const int quads = (len + 4 * kRankThreads - 1) / (4 * kRankThreads), run = quads * 256;
+  const int first = wave * run + 4 * lane;
+  struct Four {
+    float x[4];
+  };
+  auto load = [&](int r) {  // 16 bytes, on any float's boundary; capacities are whole blocks
+    const int i = first + 256 * r;
+    Four v;
+    __builtin_memcpy(&v, w + (r < quads && i < old ? i : 0), sizeof(v));
+    return v;
+  };
+  auto keys = [&](int r, const Four& v) {
+    const int i = first + 256 * r;
+    u32x4 k;
 #pragma unroll
-    for (int q = 0; q < n; ++q) {
-      const int i = first + 64 * (r0 + q);
-      x[q] = w[i < old ? i : 0];  // capacity > 0
-    }
-#pragma unroll
-    for (int q = 0; q < n; ++q) {
-      const int i = first + 64 * (r0 + q);
-      k[q] = r0 + q >= per ? 0u : i < old ? rank_bits(x[q]) : i < len ? kAlways : 0u;
-    }
+    for (int q = 0; q < 4; ++q) k[q] = i + q < old ? rank_bits(v.x[q]) : i + q < len ? kAlways : 0u;
+    return k;
   };
   if constexpr (N > 0) {
-    for (int r = 0; r < per; r += 8) {
-      uint32_t k[8];
-      keys(r, k);
+    for (int r = 0; r < quads; r += 8) {  // eight loads under way together
+      Four v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = load(r + q);
 #pragma unroll
       for (int q = 0; q < 8; ++q)
-        if (r + q < per) held[first + 64 * (r + q)] = k[q];  // read by the same lane alone
+        if (r + q < quads)  // read by the same lane alone
+          *reinterpret_cast<u32x4*>(&held[first + 256 * (r + q)]) = keys(r + q, v[q]);
     }
   }
-  // f(i, key) for every token of this lane; key 0 behind the last.
+  // f(i, the keys of tokens i .. i + 3) for every token of this lane; key 0 behind the last.
   auto each = [&](auto f) {
-    for (int r = 0; r < per; r += 4) {
-      uint32_t k[4];
-      if constexpr (N > 0) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) k[q] = held[first + 64 * (r + q)];
-#pragma unroll
-        for (int q = 1; q < 4; ++q) k[q] = r + q < per ? k[q] : 0u;
-      } else {
-        keys(r, k);
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) f(first + 64 * (r + q), k[q]);
+    for (int r = 0; r < quads; ++r) {
+      const int i = first + 256 * r;
+      if constexpr (N > 0) f(i, *reinterpret_cast<const u32x4*>(&held[i]));
+      else f(i, keys(r, load(r)));
     }
   };
 
@@ -113,8 +108,10 @@ __global__ __launch_bounds__(kRankThreads) void rank_kernel(const int32_t* lengt
       while ((z - a - 1) >> shift >= kBins) ++shift;
       reinterpret_cast<u32x4*>(bins)[tid] = u32x4{0u, 0u, 0u, 0u};
       __syncthreads();
-      each([&](int, uint32_t k) {
-        if (k >= a && k < z) atomicAdd(&bins[(k - (uint32_t)a) >> shift], 1u);
+      each([&](int, u32x4 k) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (k[q] >= a && k[q] < z) atomicAdd(&bins[(k[q] - (uint32_t)a) >> shift], 1u);
       });
       __syncthreads();
       // Thread t: bins 4 t .. 4 t + 3, and how many keys lie in the bins behind them.
@@ -145,8 +142,10 @@ __global__ __launch_bounds__(kRankThreads) void rank_kernel(const int32_t* lengt
       if (tid < (int)kLast) bins[tid] = 0;
       if (tid == 0) found[0] = 0;
       __syncthreads();
-      each([&](int, uint32_t k) {
-        if (k >= a && k < z) bins[atomicAdd(&found[0], 1u)] = k;  // in any order
+      each([&](int, u32x4 k) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (k[q] >= a && k[q] < z) bins[atomicAdd(&found[0], 1u)] = k[q];  // in any order
       });
       __syncthreads();
       if (tid < (int)have) {
@@ -172,9 +171,12 @@ __global__ __launch_bounds__(kRankThreads) void rank_kernel(const int32_t* lengt
   }
   // Where this wave's tokens go, and which ties are its own.
   uint32_t n_new = 0, n_tie = 0;
-  each([&](int, uint32_t k) {
-    n_new += k > T ? 1u : 0u;
-    n_tie += k == T ? 1u : 0u;  // counted only where there are ties
+  each([&](int, u32x4 k) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      n_new += k[q] > T ? 1u : 0u;
+      n_tie += k[q] == T ? 1u : 0u;  // counted only where there are ties
+    }
   });
   for (int o = 1; o < 64; o <<= 1) n_new += __shfl_xor(n_new, o), n_tie += __shfl_xor(n_tie, o);
   __syncthreads();  // waves is read
@@ -187,23 +189,39 @@ __global__ __launch_bounds__(kRankThreads) void rank_kernel(const int32_t* lengt
     tie += use;
   }
   int32_t* list = kept + (int64_t)bh * keep;
-  if (ties == 0) {
-    each([&](int i, uint32_t k) {
-      const uint64_t mask = __ballot(k > T);
-      if (k > T) list[at + mbcnt64(mask)] = i;
+  each([&](int i, u32x4 k) {
+    bool stay[4];
+    if (ties == 0) {  // workgroup-uniform
+#pragma unroll
+      for (int q = 0; q < 4; ++q) stay[q] = k[q] > T;
+    } else {
+      uint32_t before = tie, all = 0;  // ties of the lanes before, and of this lane so far
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint64_t mask = __ballot(k[q] == T);
+        before += mbcnt64(mask);
+        all += (uint32_t)__popcll(mask);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        stay[q] = k[q] > T || (k[q] == T && before < ties);
+        before += k[q] == T ? 1u : 0u;
+      }
+      tie = tie + all < ties ? tie + all : ties;
+    }
+    uint32_t to = at;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint64_t mask = __ballot(stay[q]);
+      to += mbcnt64(mask);
       at += (uint32_t)__popcll(mask);
-    });
-  } else {
-    each([&](int i, uint32_t k) {
-      const uint64_t tie_mask = __ballot(k == T);
-      const bool stay = k > T || (k == T && tie + mbcnt64(tie_mask) < ties);
-      const uint64_t mask = __ballot(stay);
-      if (stay) list[at + mbcnt64(mask)] = i;
-      at += (uint32_t)__popcll(mask);
-      tie += (uint32_t)__popcll(tie_mask);
-      tie = tie < ties ? tie : ties;
-    });
-  }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (stay[q]) list[to] = i + q;
+      to += stay[q] ? 1u : 0u;
+    }
+  });
   for (int i = left + tid; i < keep; i += kRankThreads) list[i] = -1;
   if (tid == 0 && bh % H == 0) new_lengths[b] = left;
 }
@@ -271,7 +289,8 @@ __global__ __launch_bounds__(256) void gather_kernel(Cache8 src, Cache8 dst, con
     for (int i = 0; i < 4 * W; ++i) byte[i] = in[i * 64];
 #pragma unroll
     for (int i = 0; i < W; ++i)
-      vw[i] = byte[4 * i] | (uint32_t)byte[4 * i + 1] << 8 | (uint32_t)byte[4 * i + 2] << 16 | (uint32_t)byte[4 * i + 3] << 24;
+      vw[i] = byte[4 * i] | (uint32_t)byte[4 * i + 1] << 8 | (uint32_t)byte[4 * i + 2] << 16 |
+              (uint32_t)byte[4 * i + 3] << 24;
     vs = src.v_scale[old + vt / 64];
     if (wave == 0) weight = weights[old * 64 + vt];
   }
@@ -308,11 +327,11 @@ void launch_rank(const Cache8& src, const int32_t* lengths, const float* weights
 hipError_t launch_cache_evict(const Cache8& src, const int32_t* lengths, const float* weights, int keep, int recent,
                               const Cache8& dst, float* w_out, int32_t* kept, int32_t* new_lengths, int D,
                               hipStream_t stream) {
-  const int64_t most = ((int64_t)src.nb * 64 + kRankThreads - 1) / kRankThreads * kRankThreads;
+  const int64_t most = (int64_t)src.nb * 64;  // LDS holds whole rounds of 4096
   // Weights in LDS up to what it holds (32 heads of 18,720 tokens: the call 67 us, read anew
   // 78; 8 heads of 32,000 and 20,000: 41 and 63), and little of it where little is needed, for
-  // two workgroups a CU (8 times 64 heads of 4000 tokens: 67 us, with all of it 72).
-  const auto rank = most <= 4096 ? launch_rank<4096> : most <= 35840 ? launch_rank<35840> : launch_rank<0>;
+  // two workgroups a CU (8 times 64 heads of 4000 tokens: 67 us, with 35,840's room 72).
+  const auto rank = most <= 4096 ? launch_rank<4096> : most <= 32768 ? launch_rank<32768> : launch_rank<0>;
   rank(src, lengths, weights, keep, recent, kept, new_lengths, stream);
   const uint32_t grid = (uint32_t)((int64_t)src.B * src.H * dst.nb);
   if (D == 64)
