@@ -2,9 +2,9 @@
 // number of query rows, grouped heads, ragged lengths read on the device, and a
 // causal mask among an item's queries.
 //
-// The stored bytes go to the matrix cores as T, exactly; a block's scales are powers
-// of two and enter where they round nothing.  With u = score * log2(e), a block's key
-// scale multiplies u, and its value scale 2^ev is added to the exponent:
+// The stored bytes go to the matrix cores exactly, as T or as they are; a block's scales
+// are powers of two and enter where they round nothing.  With u = score * log2(e), a
+// block's key scale multiplies u, and its value scale 2^ev is added to the exponent:
 //   P' = exp2(u + ev - m),  m the running maximum of u + ev,
 //   O  = sum P' v8,         l = sum 2^-ev P',
 // so P' <= 1 in any mix of scales, O holds the true sum over 2^m, and l the softmax's
@@ -467,14 +467,41 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 //
 // Bound by instructions: a block costs a wave 64 MFMAs (1024 cycles), 32 exponentials with
 // their sums and 128 conversions of bytes, about 2350 cycles with the MFMAs beside them.
-// 12,480 queries of 32 heads of 128 over 18,720 tokens take 3.6 ms, 1062 TFLOP/s in bf16,
-// where a product of 8192^3 makes 1214.  D = 128 leaves registers for three waves a SIMD
-// (two: 3804 us, three 3580 then), D = 64 for four (4000 queries of 16 heads over 9000
-// tokens 195 us, three 200).
+// D = 128 leaves registers for three waves a SIMD (12,480 queries of 32 heads over 18,720
+// tokens: two 3804 us, three 3580), D = 64 for four (4000 queries of 16 heads over 9000
+// tokens: 195 us, three 200).
+//
+// kBytes (bf16, D = 128, long walks): the keys' bytes go to 16 x 16 x 128 MFMAs as they are,
+// and a row's values as the sum of two e4m3 numbers under the row's 2^e and 2^(e - 4): two
+// passes at twice bf16's rate, and 64 conversions less.  e4m3's 4 bits twice are bf16's 8,
+// so that values of 2^-14.8 of the row's largest and more are exact, and those below within
+// 2^-22 of the largest.  Where more than kSmall of a lane's 64 values are not held to 2^-12
+// of themselves (a row whose largest is far above the rest, which its keys may not answer;
+// normally distributed rows have 0.1 a lane), the workgroup converts the keys instead.
+// 12,480 queries of 32 heads over 18,720 tokens then take 3376 us, 1134 TFLOP/s, against
+// 3637 (a product of 8192^3 makes 1214); 2048 over 2048 of 32 heads 75 against 78.
 template <typename T>
 constexpr float kMaxSum = 0x1p40f;
 template <>
 constexpr float kMaxSum<f16> = 0x1p15f;
+
+template <typename T>
+constexpr bool kIsBf16 = false;
+template <>
+constexpr bool kIsBf16<bf16> = true;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+constexpr int kSmall = 4;
+
+// The least e >= -123 with |q| <= 448 2^e = 1.75 2^(e + 8) in the lane's row, of which it
+// holds a quarter.
+template <int D, typename V>
+__device__ __forceinline__ int byte_exponent(const V (&q)[D / 32]) {
+  float amax = 0.0f;
+#pragma unroll
+  for (int x = 0; x < D / 4; ++x) amax = fmaxf(amax, __builtin_fabsf(to_f32(q[x / 8][x % 8])));
+  const int e = (int)((__builtin_bit_cast(uint32_t, max_quarters(amax)) + 0x1fffffu) >> 23) - 135;
+  return e < -123 ? -123 : e;
+}
 
 template <int D>
 struct Tile8 {
@@ -483,7 +510,7 @@ struct Tile8 {
   __device__ static int vswz(int d) { return (d >> 2) & 3; }
 };
 
-template <typename T, int D>
+template <typename T, int D, bool kBytes>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 128 ? 3 : 4, D == 128 ? 3 : 4)))
 void many_rows_kernel(CacheAttn a, Parts p) {
   typedef typename Mfma<T>::vec8 vec8;
@@ -527,294 +554,353 @@ void many_rows_kernel(CacheAttn a, Parts p) {
           vec8, vis[qt] > 0 ? *reinterpret_cast<const u32x4*>(q + 8 * ks) : u32x4{0u, 0u, 0u, 0u});
   }
   __shared__ int wave_dirty[4];
-
-  const uint32_t head_bytes = (uint32_t)a.c.nb * (uint32_t)kHalf;  // capacities are limited so that this fits
-  const uint8_t* vhead = a.c.v8 + (int64_t)bh * a.c.nb * kHalf;
-  const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
-      a.c.k8 + (int64_t)bh * a.c.nb * kHalf, (short)0, (int)head_bytes, kBufferFlags);
-  const __amdgpu_buffer_rsrc_t vrs =
-      __builtin_amdgcn_make_buffer_rsrc((void*)vhead, (short)0, (int)head_bytes, kBufferFlags);
-  uint32_t ko[kLoads], vo[kLoads];
+  auto rest = [&](auto form) __attribute__((always_inline)) {
+    constexpr bool bytes = decltype(form)::value;
+    i32x8 q8[2][2];  // [query tile][first, rest]
+    int q8_scale[2];
+    if constexpr (bytes) {
 #pragma unroll
-  for (int u = 0; u < kLoads; ++u) {
-    const int slot = 64 * (kLoads * wave + u) + lane;  // 16-byte chunk of the block
-    const int kr = slot / C::kKeyChunks, kc = slot % C::kKeyChunks;
-    ko[u] = 16u * (uint32_t)(kr * C::kKeyChunks + (kc ^ C::kswz(kr)));
-    const int vr = slot / 4, vc = slot % 4;
-    vo[u] = 16u * (uint32_t)(vr * 4 + (vc ^ C::vswz(vr)));
-  }
-  auto fetch = [&](int j, int slot) {
-    const uint32_t m0 = lds_addr(ring + slot * kSlot + 1024 * (kLoads * wave));
-    const int off = (int)((uint32_t)j * (uint32_t)kHalf);
+      for (int qt = 0; qt < 2; ++qt) {
+        const int e = byte_exponent<D>(qf[qt]);
+        const float inv = pow2i(-e);
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) dma16_settled(krs, ko[u], off, m0 + 1024u * u);
+        for (int w = 0; w < D / 16; ++w) {
+          float x[4], y[4];
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) dma16_settled(vrs, vo[u], off, m0 + kHalf + 1024u * u);
-  };
-
-  // The scales of 64 blocks at a time: lane l holds block base + l's.
-  const float* ksc = a.c.k_scale + (int64_t)bh * a.c.nb;
-  const float* vsc = a.c.v_scale + (int64_t)bh * a.c.nb;
-  float ks64 = 0.0f, vs64 = 0.0f;
-  auto scales = [&](int base) {
-    const int j = base + lane < a.c.nb ? base + lane : a.c.nb - 1;
-    ks64 = ksc[j];
-    vs64 = vsc[j];
-  };
-
-  // A block's keys go in two halves: half h of lane group G is keys 16 G + 8 (h ^ G % 2)
-  // .. + 7 (the groups alternate, so that the 8 bytes that a half reads of each of v8's
-  // chunks lie in all banks), two key tiles of 4 a group.
-  const int hk = 8 * (G & 1), hr = 8 * ((gi / 4) & 1);
-  int kaddr[2][D / 64], vaddr[2];
+          for (int i = 0; i < 4; ++i) x[i] = to_f32(qf[qt][w / 2][4 * (w % 2) + i]) * inv;
+          const uint32_t word = pack_e4m3(x[0], x[1], x[2], x[3]);
+          unpack_e4m3(word, y);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int row = 16 * (gi / 4) + (hr ^ (8 * h)) + gi % 4;  // its swizzle is that of the lane, whatever the tile
-#pragma unroll
-    for (int u = 0; u < D / 64; ++u) kaddr[h][u] = row * D + 16 * ((G * (D / 64) + u) ^ C::kswz(row));
-    vaddr[h] = kHalf + gi * 64 + 16 * (G ^ C::vswz(gi)) + (hk ^ (8 * h));
-  }
-
-  f32x4 o[D / 16][2];
-  float m[2], l[2];
-  bool nan_found = false;
-
-  f32x4 s[2][2][2];  // [half][key tile][query tile]
-  vec8 pf[2][2];     // [half][query tile]
-  float sum[2];
-  auto qk = [&](const uint8_t* tile8, int h) {
-    constexpr int kReads = 2 * (D / 64);  // read r: key tile r / (D / 64), chunk r % (D / 64)
-    u32x4 kw[kReads];
-#pragma unroll
-    for (int r = 0; r < kReads; ++r)
-      kw[r] = *reinterpret_cast<const u32x4*>(tile8 + kaddr[h][r % (D / 64)] + 4 * (r / (D / 64)) * D);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) s[h][t][0] = s[h][t][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int r = 0; r < kReads; ++r) {
-      const int t = r / (D / 64), u = r % (D / 64);
-      const vec8 k0 = From8<T>::cvt(kw[r][0], kw[r][1]), k1 = From8<T>::cvt(kw[r][2], kw[r][3]);
-      s[h][t][0] = Mfma<T>::mma(k0, qf[0][2 * u], s[h][t][0]);
-      s[h][t][1] = Mfma<T>::mma(k0, qf[1][2 * u], s[h][t][1]);
-      s[h][t][0] = Mfma<T>::mma(k1, qf[0][2 * u + 1], s[h][t][0]);
-      s[h][t][1] = Mfma<T>::mma(k1, qf[1][2 * u + 1], s[h][t][1]);
-    }
-  };
-  auto mask = [&](int j, int h) {
-#pragma unroll
-    for (int qt = 0; qt < 2; ++qt) {
-      const int left = here(vis[qt] - 64 * j - 16 * G - (hk ^ (8 * h)));
-#pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (x >= left) s[h][x / 4][qt][x % 4] = kNegInf;
-    }
-  };
-  auto row_max = [&](int h, int qt) {
-    float mx = s[h][0][qt][0];
-#pragma unroll
-    for (int x = 1; x < 8; ++x) mx = __builtin_elementwise_maximum(mx, s[h][x / 4][qt][x % 4]);
-    return max_quarters(mx);
-  };
-  auto raise = [&](int h, float c, float ev) {
-#pragma unroll
-    for (int qt = 0; qt < 2; ++qt) m[qt] = __builtin_elementwise_maximum(m[qt], __builtin_fmaf(row_max(h, qt), c, ev));
-  };
-  auto key_scale = [&](int j) {
-    const float c = a.scale_log2 * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks64), j & 63));
-    return c > 0x1p-126f ? c : 0x1p-126f;  // so that a masked score of -inf times c is -inf
-  };
-  auto exps = [&](int h, float c, float ev) {
-#pragma unroll
-    for (int qt = 0; qt < 2; ++qt) {
-      const float off = m[qt] == kNegInf ? ev : ev - m[qt];
-      sum[qt] = 0.0f;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const float p = fast_exp2(__builtin_fmaf(s[h][x / 4][qt][x % 4], c, off));
-        sum[qt] += p;
-        pf[h][qt][x] = from_f32<T>(p);
+          for (int i = 0; i < 4; ++i) y[i] = (x[i] - y[i]) * 16.0f;
+          q8[qt][0][w] = (int)word;
+          q8[qt][1][w] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3],
+                                                        __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), true);
+        }
+        q8_scale[qt] = e + 127;
       }
     }
-  };
-  auto pv = [&](const uint8_t* tile8, int h) {
-#pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) {
-      const u32x2 w = *reinterpret_cast<const u32x2*>(tile8 + vaddr[h] + dt * (16 * 64));
-      const vec8 v = From8<T>::cvt(w[0], w[1]);
-      o[dt][0] = Mfma<T>::mma(v, pf[h][0], o[dt][0]);
-      o[dt][1] = Mfma<T>::mma(v, pf[h][1], o[dt][1]);
-    }
-  };
-  // The same where some row sees the block in part: NaN count as zero here, and are put
-  // where they belong at the end.
-  auto pv_part = [&](const uint8_t* tile8, int h) {
-    uint32_t bad = 0;
-#pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) {
-      u32x2 w = *reinterpret_cast<const u32x2*>(tile8 + vaddr[h] + dt * (16 * 64));
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint32_t nan = nan_bytes(w[x]);
-        bad |= nan;
-        w[x] &= ~((nan - (nan >> 7)) | nan);
-      }
-      const vec8 v = From8<T>::cvt(w[0], w[1]);
-      o[dt][0] = Mfma<T>::mma(v, pf[h][0], o[dt][0]);
-      o[dt][1] = Mfma<T>::mma(v, pf[h][1], o[dt][1]);
-    }
-    if (__ballot(bad != 0)) nan_found = true;
-  };
 
-  bool dirty = false, exact = false;
-  auto block = [&](int j, int slot, auto kind) {
-    constexpr bool part = decltype(kind)::value;  // some row of the wave sees the block in part
-    const uint8_t* tile8 = ring + slot * kSlot;
-    const float c = key_scale(j);
-    const int e = exponent_of(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs64), j & 63)));
-    const float ev = (float)e, unit = pow2i(-e);
+    const uint32_t head_bytes = (uint32_t)a.c.nb * (uint32_t)kHalf;  // capacities are limited so that this fits
+    const uint8_t* vhead = a.c.v8 + (int64_t)bh * a.c.nb * kHalf;
+    const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
+        a.c.k8 + (int64_t)bh * a.c.nb * kHalf, (short)0, (int)head_bytes, kBufferFlags);
+    const __amdgpu_buffer_rsrc_t vrs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)vhead, (short)0, (int)head_bytes, kBufferFlags);
+    uint32_t ko[kLoads], vo[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int slot = 64 * (kLoads * wave + u) + lane;  // 16-byte chunk of the block
+      const int kr = slot / C::kKeyChunks, kc = slot % C::kKeyChunks;
+      ko[u] = 16u * (uint32_t)(kr * C::kKeyChunks + (kc ^ C::kswz(kr)));
+      const int vr = slot / 4, vc = slot % 4;
+      vo[u] = 16u * (uint32_t)(vr * 4 + (vc ^ C::vswz(vr)));
+    }
+    auto fetch = [&](int j, int slot) {
+      const uint32_t m0 = lds_addr(ring + slot * kSlot + 1024 * (kLoads * wave));
+      const int off = (int)((uint32_t)j * (uint32_t)kHalf);
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) dma16_settled(krs, ko[u], off, m0 + 1024u * u);
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) dma16_settled(vrs, vo[u], off, m0 + kHalf + 1024u * u);
+    };
+
+    // The scales of 64 blocks at a time: lane l holds block base + l's.
+    const float* ksc = a.c.k_scale + (int64_t)bh * a.c.nb;
+    const float* vsc = a.c.v_scale + (int64_t)bh * a.c.nb;
+    float ks64 = 0.0f, vs64 = 0.0f;
+    auto scales = [&](int base) {
+      const int j = base + lane < a.c.nb ? base + lane : a.c.nb - 1;
+      ks64 = ksc[j];
+      vs64 = vsc[j];
+    };
+
+    // A block's keys go in two halves: half h of lane group G is keys 16 G + 8 (h ^ G % 2)
+    // .. + 7 (the groups alternate, so that the 8 bytes that a half reads of each of v8's
+    // chunks lie in all banks), two key tiles of 4 a group.
+    const int hk = 8 * (G & 1), hr = 8 * ((gi / 4) & 1);
+    int kaddr[2][D / 64], vaddr[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      qk(tile8, h);
-      if constexpr (part) mask(j, h);
-      if (h == 0 && j == j0 && !exact) raise(h, c, ev);
-      exps(h, c, ev);
-      if (__ballot(!(sum[0] <= kMaxSum<T> && sum[1] <= kMaxSum<T>))) dirty = true;
-      l[0] = __builtin_fmaf(sum[0], unit, l[0]);
-      l[1] = __builtin_fmaf(sum[1], unit, l[1]);
-      if constexpr (part) pv_part(tile8, h);
-      else pv(tile8, h);
-    }
-  };
-  // Blocks before `whole` are seen whole by every row of the wave that sees any token.
-  const int whole = own == 0 ? 0 : least / 64 < j1 ? least / 64 : j1;
-  int j, slot;
-  auto begin = [&] {
-    j = j0, slot = 0;
-    scales(j0 & ~63);
-    fetch(j0, 0);
-    if (j0 + 1 < j1) fetch(j0 + 1, 1);
-  };
-  auto next = [&] {
-    if (j + 1 < j1) wait_vmcnt<2 * kLoads>();
-    else wait_vmcnt<0>();
-    __syncthreads();  // block j has landed, and the one before it is read by all
-    if ((j & 63) == 0 && j > j0) scales(j);
-    if (j + 2 < j1) fetch(j + 2, slot == 0 ? 2 : slot - 1);
-  };
-  m[0] = m[1] = kNegInf;
-  for (;;) {
-    l[0] = l[1] = 0.0f;
+      const int row = 16 * (gi / 4) + (hr ^ (8 * h)) + gi % 4;  // its swizzle is that of the lane, whatever the tile
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-      for (int qt = 0; qt < 2; ++qt) o[dt][qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (j0 >= j1) break;
-    begin();
-    for (; j < whole; ++j) {
-      next();
-      block(j, slot, Flag<false>{});
-      slot = slot == 2 ? 0 : slot + 1;
+      for (int u = 0; u < D / 64; ++u) kaddr[h][u] = row * D + 16 * ((G * (D / 64) + u) ^ C::kswz(row));
+      vaddr[h] = kHalf + gi * 64 + 16 * (G ^ C::vswz(gi)) + (hk ^ (8 * h));
     }
-    for (; j < j1; ++j) {
-      next();
-      if (64 * j < own) block(j, slot, Flag<true>{});
-      slot = slot == 2 ? 0 : slot + 1;
-    }
-    if (lane == 0) wave_dirty[wave] = dirty ? 1 : 0;
-    __syncthreads();  // the ring is free, the flags are there
-    if (exact || !(wave_dirty[0] | wave_dirty[1] | wave_dirty[2] | wave_dirty[3])) break;  // workgroup-uniform
-    exact = true;
-    begin();
-    for (; j < j1; ++j, slot = slot == 2 ? 0 : slot + 1) {  // the rows' maxima
-      next();
-      if (64 * j >= own) continue;
-      const float c = key_scale(j);
-      const float ev = (float)exponent_of(
-          __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs64), j & 63)));
+
+    f32x4 o[D / 16][2];
+    float m[2], l[2];
+    bool nan_found = false;
+
+    f32x4 s[2][2][2];  // [half][key tile][query tile]
+    vec8 pf[2][2];     // [half][query tile]
+    float sum[2];
+    auto qk = [&](const uint8_t* tile8, int h) {
+      constexpr int kReads = 2 * (D / 64);  // read r: key tile r / (D / 64), chunk r % (D / 64)
+      u32x4 kw[kReads];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        qk(ring + slot * kSlot, h);
-        if (j >= whole) mask(j, h);
-        raise(h, c, ev);
+      for (int r = 0; r < kReads; ++r)
+        kw[r] = *reinterpret_cast<const u32x4*>(tile8 + kaddr[h][r % (D / 64)] + 4 * (r / (D / 64)) * D);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[h][t][0] = s[h][t][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (bytes) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          i32x8 k;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) k[x] = (int)kw[2 * t + x / 4][x % 4];
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int qt = 0; qt < 2; ++qt)
+              s[h][t][qt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                  k, q8[qt][part], s[h][t][qt], 0, 0, 0, 127, 0, q8_scale[qt] - 4 * part);
+        }
+        return;
       }
-    }
-    __syncthreads();
-  }
-  if (nan_found) {  // wave-uniform, rare: rows that see a NaN among the values get one
-    for (int j = whole > j0 ? whole : j0; j < j1 && 64 * j < own; ++j) {
-      const uint8_t* vj = vhead + (int64_t)j * kHalf + gi * 64 + 16 * G;
-      vec8 seen[2][2];
+#pragma unroll
+      for (int r = 0; r < kReads; ++r) {
+        const int t = r / (D / 64), u = r % (D / 64);
+        const vec8 k0 = From8<T>::cvt(kw[r][0], kw[r][1]), k1 = From8<T>::cvt(kw[r][2], kw[r][3]);
+        s[h][t][0] = Mfma<T>::mma(k0, qf[0][2 * u], s[h][t][0]);
+        s[h][t][1] = Mfma<T>::mma(k0, qf[1][2 * u], s[h][t][1]);
+        s[h][t][0] = Mfma<T>::mma(k1, qf[0][2 * u + 1], s[h][t][0]);
+        s[h][t][1] = Mfma<T>::mma(k1, qf[1][2 * u + 1], s[h][t][1]);
+      }
+    };
+    auto mask = [&](int j, int h) {
+#pragma unroll
+      for (int qt = 0; qt < 2; ++qt) {
+        const int left = here(vis[qt] - 64 * j - 16 * G - (hk ^ (8 * h)));
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if (x >= left) s[h][x / 4][qt][x % 4] = kNegInf;
+      }
+    };
+    auto row_max = [&](int h, int qt) {
+      float mx = s[h][0][qt][0];
+#pragma unroll
+      for (int x = 1; x < 8; ++x) mx = __builtin_elementwise_maximum(mx, s[h][x / 4][qt][x % 4]);
+      return max_quarters(mx);
+    };
+    auto raise = [&](int h, float c, float ev) {
 #pragma unroll
       for (int qt = 0; qt < 2; ++qt)
+        m[qt] = __builtin_elementwise_maximum(m[qt], __builtin_fmaf(row_max(h, qt), c, ev));
+    };
+    auto key_scale = [&](int j) {
+      const float c = a.scale_log2 * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks64), j & 63));
+      return c > 0x1p-126f ? c : 0x1p-126f;  // so that a masked score of -inf times c is -inf
+    };
+    auto exps = [&](int h, float c, float ev) {
 #pragma unroll
-        for (int x = 0; x < 16; ++x)
-          seen[x / 8][qt][x % 8] = from_f32<T>(64 * j + 16 * G + x < vis[qt] ? 1.0f : 0.0f);
+      for (int qt = 0; qt < 2; ++qt) {
+        const float off = m[qt] == kNegInf ? ev : ev - m[qt];
+        sum[qt] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float p = fast_exp2(__builtin_fmaf(s[h][x / 4][qt][x % 4], c, off));
+          sum[qt] += p;
+          pf[h][qt][x] = from_f32<T>(p);
+        }
+      }
+    };
+    auto pv = [&](const uint8_t* tile8, int h) {
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt) {
-        u32x4 is = *reinterpret_cast<const u32x4*>(vj + dt * (16 * 64));
+        const u32x2 w = *reinterpret_cast<const u32x2*>(tile8 + vaddr[h] + dt * (16 * 64));
+        const vec8 v = From8<T>::cvt(w[0], w[1]);
+        o[dt][0] = Mfma<T>::mma(v, pf[h][0], o[dt][0]);
+        o[dt][1] = Mfma<T>::mma(v, pf[h][1], o[dt][1]);
+      }
+    };
+    // The same where some row sees the block in part: NaN count as zero here, and are put
+    // where they belong at the end.
+    auto pv_part = [&](const uint8_t* tile8, int h) {
+      uint32_t bad = 0;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) is[x] = nan_bytes(is[x]) >> 7 << 3;  // a positive number for each NaN
-        const vec8 i0 = From8<T>::cvt(is[0], is[1]), i1 = From8<T>::cvt(is[2], is[3]);
+      for (int dt = 0; dt < D / 16; ++dt) {
+        u32x2 w = *reinterpret_cast<const u32x2*>(tile8 + vaddr[h] + dt * (16 * 64));
 #pragma unroll
-        for (int qt = 0; qt < 2; ++qt) {
-          f32x4 hit = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          hit = Mfma<T>::mma(i0, seen[0][qt], hit);
-          hit = Mfma<T>::mma(i1, seen[1][qt], hit);
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t nan = nan_bytes(w[x]);
+          bad |= nan;
+          w[x] &= ~((nan - (nan >> 7)) | nan);
+        }
+        const vec8 v = From8<T>::cvt(w[0], w[1]);
+        o[dt][0] = Mfma<T>::mma(v, pf[h][0], o[dt][0]);
+        o[dt][1] = Mfma<T>::mma(v, pf[h][1], o[dt][1]);
+      }
+      if (__ballot(bad != 0)) nan_found = true;
+    };
+
+    bool dirty = false, exact = false;
+    auto block = [&](int j, int slot, auto kind) {
+      constexpr bool part = decltype(kind)::value;  // some row of the wave sees the block in part
+      const uint8_t* tile8 = ring + slot * kSlot;
+      const float c = key_scale(j);
+      const int e = exponent_of(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs64), j & 63)));
+      const float ev = (float)e, unit = pow2i(-e);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (hit[i] > 0.0f) o[dt][qt][i] = __builtin_nanf("");
+      for (int h = 0; h < 2; ++h) {
+        qk(tile8, h);
+        if constexpr (part) mask(j, h);
+        if (h == 0 && j == j0 && !exact) raise(h, c, ev);
+        exps(h, c, ev);
+        if (__ballot(!(sum[0] <= kMaxSum<T> && sum[1] <= kMaxSum<T>))) dirty = true;
+        l[0] = __builtin_fmaf(sum[0], unit, l[0]);
+        l[1] = __builtin_fmaf(sum[1], unit, l[1]);
+        if constexpr (part) pv_part(tile8, h);
+        else pv(tile8, h);
+      }
+    };
+    // Blocks before `whole` are seen whole by every row of the wave that sees any token.
+    const int whole = own == 0 ? 0 : least / 64 < j1 ? least / 64 : j1;
+    int j, slot;
+    auto begin = [&] {
+      j = j0, slot = 0;
+      scales(j0 & ~63);
+      fetch(j0, 0);
+      if (j0 + 1 < j1) fetch(j0 + 1, 1);
+    };
+    auto next = [&] {
+      if (j + 1 < j1) wait_vmcnt<2 * kLoads>();
+      else wait_vmcnt<0>();
+      __syncthreads();  // block j has landed, and the one before it is read by all
+      if ((j & 63) == 0 && j > j0) scales(j);
+      if (j + 2 < j1) fetch(j + 2, slot == 0 ? 2 : slot - 1);
+    };
+    m[0] = m[1] = kNegInf;
+    for (;;) {
+      l[0] = l[1] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+        for (int qt = 0; qt < 2; ++qt) o[dt][qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (j0 >= j1) break;
+      begin();
+      for (; j < whole; ++j) {
+        next();
+        block(j, slot, Flag<false>{});
+        slot = slot == 2 ? 0 : slot + 1;
+      }
+      for (; j < j1; ++j) {
+        next();
+        if (64 * j < own) block(j, slot, Flag<true>{});
+        slot = slot == 2 ? 0 : slot + 1;
+      }
+      if (lane == 0) wave_dirty[wave] = dirty ? 1 : 0;
+      __syncthreads();  // the ring is free, the flags are there
+      if (exact || !(wave_dirty[0] | wave_dirty[1] | wave_dirty[2] | wave_dirty[3])) break;  // workgroup-uniform
+      exact = true;
+      begin();
+      for (; j < j1; ++j, slot = slot == 2 ? 0 : slot + 1) {  // the rows' maxima
+        next();
+        if (64 * j >= own) continue;
+        const float c = key_scale(j);
+        const float ev = (float)exponent_of(
+            __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs64), j & 63)));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          qk(ring + slot * kSlot, h);
+          if (j >= whole) mask(j, h);
+          raise(h, c, ev);
+        }
+      }
+      __syncthreads();
+    }
+    if (nan_found) {  // wave-uniform, rare: rows that see a NaN among the values get one
+      for (int j = whole > j0 ? whole : j0; j < j1 && 64 * j < own; ++j) {
+        const uint8_t* vj = vhead + (int64_t)j * kHalf + gi * 64 + 16 * G;
+        vec8 seen[2][2];
+#pragma unroll
+        for (int qt = 0; qt < 2; ++qt)
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            seen[x / 8][qt][x % 8] = from_f32<T>(64 * j + 16 * G + x < vis[qt] ? 1.0f : 0.0f);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+          u32x4 is = *reinterpret_cast<const u32x4*>(vj + dt * (16 * 64));
+#pragma unroll
+          for (int x = 0; x < 4; ++x) is[x] = nan_bytes(is[x]) >> 7 << 3;  // a positive number for each NaN
+          const vec8 i0 = From8<T>::cvt(is[0], is[1]), i1 = From8<T>::cvt(is[2], is[3]);
+#pragma unroll
+          for (int qt = 0; qt < 2; ++qt) {
+            f32x4 hit = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            hit = Mfma<T>::mma(i0, seen[0][qt], hit);
+            hit = Mfma<T>::mma(i1, seen[1][qt], hit);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (hit[i] > 0.0f) o[dt][qt][i] = __builtin_nanf("");
+          }
         }
       }
     }
-  }
-  __syncthreads();  // the ring is free
+    __syncthreads();  // the ring is free
 
-  if (nblk > p.per) {
-    const int64_t part = part_at(a, p, split * a.c.B + b, kvh, 8 * tile + 2 * wave);
+    if (nblk > p.per) {
+      const int64_t part = part_at(a, p, split * a.c.B + b, kvh, 8 * tile + 2 * wave);
+#pragma unroll
+      for (int qt = 0; qt < 2; ++qt) {
+        float* po = p.o + (part + qt) * (16 * D) + gi * D + 4 * G;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt) = o[dt][qt];
+        const float all = sum_quarters(l[qt]);
+        if (G == 0) {
+          float* ml = p.ml + (part + qt) * 32 + 2 * gi;
+          ml[0] = vis[qt] > 64 * j0 ? m[qt] : kNegInf;  // a row that saw none of this part
+          ml[1] = vis[qt] > 64 * j0 ? all : 0.0f;
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
-      float* po = p.o + (part + qt) * (16 * D) + gi * D + 4 * G;
-#pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt) = o[dt][qt];
       const float all = sum_quarters(l[qt]);
-      if (G == 0) {
-        float* ml = p.ml + (part + qt) * 32 + 2 * gi;
-        ml[0] = vis[qt] > 64 * j0 ? m[qt] : kNegInf;  // a row that saw none of this part
-        ml[1] = vis[qt] > 64 * j0 ? all : 0.0f;
+      const bool empty = vis[qt] == 0 || all == 0.0f;
+      const float inv = 1.0f / all;
+      const int row = 32 * wave + 16 * qt + gi;
+      uint8_t* orow = ring + row * (2 * D);
+      const int swz = (row / (128 / D)) % (D / 8);
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) {
+        u32x2 w;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          w[x] = bits16(from_f32<T>(empty ? 0.0f : o[dt][qt][2 * x] * inv)) |
+                 (bits16(from_f32<T>(empty ? 0.0f : o[dt][qt][2 * x + 1] * inv)) << 16);
+        *reinterpret_cast<u32x2*>(orow + 16 * ((2 * dt + G / 2) ^ swz) + 8 * (G % 2)) = w;
+      }
+      const int r = kRows * tile + row;
+      if (a.lse && G == 0 && r < rows)
+        a.lse[lse_at(a, b, kvh, r)] = empty ? kNegInf : (m[qt] + __builtin_log2f(all)) * kLn2;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kRows * (D / 8) / 256; ++u) {
+      const int piece = tid + 256 * u, row = piece / (D / 8), c = piece % (D / 8);
+      const int r = kRows * tile + row;
+      if (r >= rows) continue;
+      *reinterpret_cast<u32x4*>(out_row<T>(a, b, kvh, r) + 8 * c) =
+          *reinterpret_cast<const u32x4*>(ring + row * (2 * D) + 16 * (c ^ ((row / (128 / D)) % (D / 8))));
+    }
+  };
+  if constexpr (kBytes) {
+    int small = 0;  // of the lane's 64 values, those not held to 2^-12 of themselves
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) {
+      const float bound = 0.25f * pow2i(byte_exponent<D>(qf[qt]));
+#pragma unroll
+      for (int x = 0; x < D / 4; ++x) {
+        const float y = __builtin_fabsf(to_f32(qf[qt][x / 8][x % 8]));
+        small += y != 0.0f && y < bound ? 1 : 0;
       }
     }
-    return;
-  }
-#pragma unroll
-  for (int qt = 0; qt < 2; ++qt) {
-    const float all = sum_quarters(l[qt]);
-    const bool empty = vis[qt] == 0 || all == 0.0f;
-    const float inv = 1.0f / all;
-    const int row = 32 * wave + 16 * qt + gi;
-    uint8_t* orow = ring + row * (2 * D);
-    const int swz = (row / (128 / D)) % (D / 8);
-#pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) {
-      u32x2 w;
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        w[x] = bits16(from_f32<T>(empty ? 0.0f : o[dt][qt][2 * x] * inv)) |
-               (bits16(from_f32<T>(empty ? 0.0f : o[dt][qt][2 * x + 1] * inv)) << 16);
-      *reinterpret_cast<u32x2*>(orow + 16 * ((2 * dt + G / 2) ^ swz) + 8 * (G % 2)) = w;
+    if (!__syncthreads_or(small > kSmall)) {
+      rest(Flag<true>{});
+      return;
     }
-    const int r = kRows * tile + row;
-    if (a.lse && G == 0 && r < rows)
-      a.lse[lse_at(a, b, kvh, r)] = empty ? kNegInf : (m[qt] + __builtin_log2f(all)) * kLn2;
   }
-  __syncthreads();
-#pragma unroll
-  for (int u = 0; u < kRows * (D / 8) / 256; ++u) {
-    const int piece = tid + 256 * u, row = piece / (D / 8), c = piece % (D / 8);
-    const int r = kRows * tile + row;
-    if (r >= rows) continue;
-    *reinterpret_cast<u32x4*>(out_row<T>(a, b, kvh, r) + 8 * c) =
-        *reinterpret_cast<const u32x4*>(ring + row * (2 * D) + 16 * (c ^ ((row / (128 / D)) % (D / 8))));
-  }
+  rest(Flag<false>{});
 }
 
 // Tiles of 32 rows straight from memory up to here, of 128 through LDS above.  us, 8 heads
@@ -836,6 +922,10 @@ Kind kind_of(const CacheAttn& a) {
 // two items of 1000 20 (20, 24), 2048 causal queries of 4 heads over one key head 30 (31,
 // 29).  128 walks of up to kManyOnePart 8 blocks 20.5, in two parts 23.5.
 constexpr int64_t kManyParts = 512, kManyBlocks = 6, kManyOnePart = 8;
+// Walks of up to this many blocks convert the keys (kBytes above): forming the two numbers
+// takes 1.5 us a workgroup.  1024 queries over 16 blocks 45.3 us, as bytes 45.5; walks of 8
+// 20.5 and 23.6; of 32 77.9 and 74.6, causal ones 117 and 119.
+constexpr int kLongWalk = 32;
 // us, walk and join: 256 rows 73 with a wave a row, 78 with 16 threads; 64,000 rows 212, 192.
 constexpr int64_t kJoinRows = 4096;
 
@@ -882,8 +972,11 @@ hipError_t launch(const CacheAttn& a, hipStream_t stream) {
   const int64_t each = p.tiles / (wide / 16);
   const int64_t few = ((int64_t)p.splits * a.c.H + kNumXcd - 1) / kNumXcd * kNumXcd;  // in whole rounds of the XCDs
   const dim3 grid((uint32_t)((kind == kMany ? heads * p.splits : few) * each)), threads(256);
-  if (kind == kMany)
-    hipLaunchKernelGGL((many_rows_kernel<T, D>), grid, threads, 0, stream, a, p);
+  constexpr bool bytes = kIsBf16<T> && D == 128;
+  if (kind == kMany && bytes && p.per >= kLongWalk)
+    hipLaunchKernelGGL((many_rows_kernel<T, D, bytes>), grid, threads, 0, stream, a, p);
+  else if (kind == kMany)
+    hipLaunchKernelGGL((many_rows_kernel<T, D, false>), grid, threads, 0, stream, a, p);
   else if (kind == kFew32)
     hipLaunchKernelGGL((few_rows_kernel<T, D, 2>), grid, threads, 0, stream, a, p);
   else

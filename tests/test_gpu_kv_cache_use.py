@@ -336,3 +336,45 @@ def test_moved_tensors(device):
         t.data = old.view(torch.uint8).clone().view(t.dtype)
         old.view(torch.uint8).zero_()
     assert torch.equal(cached_attention(q, c, 100), want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("kind", ["plain", "causal", "outlier", "one outlier", "sizes", "tiny", "zeros", "nan"])
+def test_long_walks(device, kind, dtype):
+    """Walks of 32 blocks of D = 128 that are not split (1024 of them): what the queries hold.
+
+    The reference's bound on a score's error, 136 2^-24 of the largest sum of |k| |q|, has
+    room for a q that is held to 2^-22 of its row's largest value where that is a few times
+    the others (2^-22 * 4 against 2^-17 of them), not where keys do not answer an outlier."""
+    from lcv_bsa import KVCache8, cache_append, cached_attention
+
+    gen = _gen(device, 3)
+    H, S, D, n = 512, 130, 128, 1999
+    k, v = (torch.randn(1, H, 2048, D, generator=gen, device=device) for _ in range(2))
+    q = torch.randn(1, H, S, D, generator=gen, device=device)
+    scale, causal = D ** -0.5, kind in ("causal", "nan")
+    if kind in ("outlier", "one outlier"):
+        k[..., 5] = 0.0
+        q[:, :, (slice(None) if kind == "outlier" else 77), 5] = 2.0 ** 15
+    elif kind == "sizes":
+        q *= torch.randn(1, 1, S, 1, generator=gen, device=device).mul_(3).exp2_()
+    elif kind == "tiny":
+        small = 2.0 ** (-110 if dtype == BF16 else -12)
+        q, scale = q * small, scale / small
+    elif kind == "zeros":
+        q *= torch.rand(q.shape, generator=gen, device=device) > 0.75
+        q[:, :, 100:120] = 0.0
+    c = cache_append(KVCache8.empty(1, H, 2048, D, device), k, v, 0)
+    if kind == "nan":
+        q[:, :, 7, 3], q[:, :, 30, 100] = math.nan, math.inf
+        c.k8.view(torch.uint8)[:, :, 1950, 3] = 127
+        c.v8.view(torch.uint8)[:, :, 31, 9, 1980 - 31 * 64] = 255
+        c.v8.view(torch.uint8)[:, :, 31, 11, 10 + n - 31 * 64] = 127  # behind the last
+    q = q.to(dtype)
+    out, lse = cached_attention(q, c, n, causal=causal, sm_scale=scale, return_lse=True)
+    for h in (0, H - 1):
+        part = KVCache8(*(t[:, h:h + 1].clone(memory_format=torch.contiguous_format) for t in (c.k8, c.v8, c.k_scale, c.v_scale)))
+        want, want_lse, tol, tol_lse, *_ = R.attention(q[:, h:h + 1], part, [n], None, causal, scale)
+        _within(out[:, h:h + 1], want, tol)
+        if kind != "nan":
+            _within(lse[:, h:h + 1], want_lse, tol_lse)
