@@ -922,9 +922,9 @@ Kind kind_of(const CacheAttn& a) {
 // two items of 1000 20 (20, 24), 2048 causal queries of 4 heads over one key head 30 (31,
 // 29).  128 walks of up to kManyOnePart 8 blocks 20.5, in two parts 23.5.
 constexpr int64_t kManyParts = 512, kManyBlocks = 6, kManyOnePart = 8;
-// Walks of up to this many blocks convert the keys (kBytes above): forming the two numbers
-// takes 1.5 us a workgroup.  1024 queries over 16 blocks 45.3 us, as bytes 45.5; walks of 8
-// 20.5 and 23.6; of 32 77.9 and 74.6, causal ones 117 and 119.
+// Walks of fewer blocks convert the keys (kBytes above): forming the two numbers takes 1.5 us
+// a workgroup.  us, 2048 queries of 32 heads over 8 key heads: over 8 blocks 29.4, as bytes
+// 31.1; over 16 45.3 and 45.5, over 32 77.9 and 74.6 (three causal prompts: 117 and 119).
 constexpr int kLongWalk = 32;
 // us, walk and join: 256 rows 73 with a wave a row, 78 with 16 threads; 64,000 rows 212, 192.
 constexpr int64_t kJoinRows = 4096;

@@ -33,7 +33,7 @@ __device__ __forceinline__ void load_keys(const CacheAttn& a, int64_t block, int
 // Few rows (up to kFewRows a key head, row r = query r / group of head r % group): a
 // pass over the keys, one block a wave; the rows come from L2, 16 at a time.  Bound by the
 // keys' bytes: one token of 4 requests over 45,480 tokens of 8 heads of 128 (49 MB) takes
-// 13.8 us, 3.6 TB/s.
+// 13.8 us, 3.6 TB/s (four waves a SIMD; with the registers of five 19.5).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void few_weights_kernel(CacheAttn a, const float* w_in, float* w_out) {
   typedef typename Mfma<T>::vec8 vec8;

@@ -122,3 +122,30 @@ def test_refusals(device):
                 m.forward_with_kv_cache(more, shape, ncl, cache)
         with pytest.raises(ValueError):
             _layer(device, heads=4, dim=64).forward_with_kv_cache(more, (3,) + GRID[1:], 2, cache)
+
+
+def test_captured_continuation(device):
+    """A denoising step captured once, replayed with other latents and another clip's cache."""
+    m = _layer(device)
+    grid = (3,) + GRID[1:]
+    with torch.no_grad():
+        x, first = _x(device, 2, 3, 256), [_x(device, 1, 2, 256, seed=s) for s in (1, 7)]
+        caches = [m(f, GRID, return_kv=True)[1] for f in first]
+        held = m(first[0], GRID, return_kv=True)[1]
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            m.forward_with_kv_cache(x, grid, 2, held)
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m.forward_with_kv_cache(x, grid, 2, held)
+        for step in range(4):
+            x.copy_(_x(device, 2, 3, 256, seed=20 + step))
+            for a, b in zip(_parts(held[0]), _parts(caches[step % 2][0])):
+                a.copy_(b)
+            graph.replay()
+            want = m.forward_with_kv_cache(x, grid, 2, caches[step % 2])
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
