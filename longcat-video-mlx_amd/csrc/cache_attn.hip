@@ -377,14 +377,26 @@ __global__ __launch_bounds__(256) void join_kernel(CacheAttn a, Parts p, int wid
   float lsum = 0.0f, acc[kN];
 #pragma unroll
   for (int e = 0; e < kN; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float f = fast_exp2(ml[i * stride * 32] - base);
-    lsum = __builtin_fmaf(ml[i * stride * 32 + 1], f, lsum);
-    float x[kN];
-    __builtin_memcpy(x, __builtin_assume_aligned(o + i * stride * (16 * D), 4 * kN > 16 ? 16 : 4 * kN), sizeof(x));
+  // So many parts' loads are under way together (past the last part it again, unused): one
+  // token of one head over 30,000 tokens 15.8 us with eight, 17.5 with four.
+  constexpr int kBatch = THREADS == 64 ? 8 : 4;
+  for (int i0 = 0; i0 < parts; i0 += kBatch) {
+    float x[kBatch][kN], m[kBatch], l[kBatch];
 #pragma unroll
-    for (int e = 0; e < kN; ++e) acc[e] = __builtin_fmaf(x[e], f, acc[e]);
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k < parts ? i0 + k : parts - 1;
+      m[k] = ml[i * stride * 32];
+      l[k] = ml[i * stride * 32 + 1];
+      __builtin_memcpy(x[k], __builtin_assume_aligned(o + i * stride * (16 * D), 4 * kN > 16 ? 16 : 4 * kN), sizeof(x[k]));
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const bool there = i0 + k < parts;
+      const float f = fast_exp2(m[k] - base);
+      lsum = there ? __builtin_fmaf(l[k], f, lsum) : lsum;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) acc[e] = there ? __builtin_fmaf(x[k][e], f, acc[e]) : acc[e];
+    }
   }
   const bool empty = top == kNegInf || visible(a, n, r / a.group) == 0;
   const float inv = 1.0f / lsum;
