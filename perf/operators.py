@@ -388,20 +388,12 @@ def _plain(s):
 # The package's operators
 # ---------------------------------------------------------------------------
 
-_lcv_bsa = None
-
-
 def _package():
-    """The package, imported once, as a user's program does."""
-    global _lcv_bsa
-    if _lcv_bsa is not None:
-        return _lcv_bsa
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "longcat-video-mlx_amd")
     if root not in sys.path:
         sys.path.insert(0, root)
     import lcv_bsa
 
-    _lcv_bsa = lcv_bsa
     return lcv_bsa
 
 
