@@ -3,16 +3,16 @@
 // causal mask among an item's queries.
 //
 // The stored bytes go to the matrix cores exactly, as T or as they are; a block's scales
-// are powers of two and enter where they round nothing.  With u = score * log2(e), a
-// block's key scale multiplies u, and its value scale 2^ev is added to the exponent:
-//   P' = exp2(u + ev - m),  m the running maximum of u + ev,
-//   O  = sum P' v8,         l = sum 2^-ev P',
-// so P' <= 1 in any mix of scales, O holds the true sum over 2^m, and l the softmax's
-// own denominator.  P' is rounded to T once, after its sum (bf16 2^-9, fp16 2^-12 relative;
-// an fp16 P' below 2^-14 loses bits only where the block with the larger values has an e4m3
-// step 2^16 times what is lost); sums, maxima and O stay in fp32.  A P' below 2^-126 is
-// zero: where value scales 2^x apart meet, each token that l then lacks has a weight below
-// 2^(x - 126); fp16's range, zeros beside it, has x = 68.
+// are powers of two and enter where they round nothing: the key scale multiplies
+// u = score * log2(e), the value scale 2^ev multiplies sums in fp32 or is added to u.
+//
+// P is rounded to T once, after its sum (bf16 2^-9, fp16 2^-12 relative), and fp16 holds
+// nothing below 2^-25.  A block of a small value scale must not get there beside one of a
+// large scale, however small its scale: what the large block stores may be zeros in all
+// channels but one.  So fp16 products are formed under one scale, or scales at most
+// kSpread apart, and P are powers above that limit.  Sums, maxima and O stay in fp32, in
+// which no mix of scales in [2^-60, 2^60] leaves the range; a token whose weight is below
+// 2^-40 of the heaviest's may be left out of the row's sum.
 //
 // The rows of one key head are its group's queries, row r = query r / group of the
 // group's head r % group; a row sees the first `vis` tokens, rows in order no fewer.  What
@@ -94,6 +94,12 @@ __device__ __forceinline__ int64_t lse_at(const CacheAttn& a, int b, int kvh, in
   return ((int64_t)b * a.c.H * a.group + kvh * a.group + r % a.group) * a.S + r / a.group;
 }
 
+// P of up to 2^kRoom: fp16 then loses what is below 2^-37 of the largest.
+template <typename T>
+constexpr int kRoom = 0;
+template <>
+constexpr int kRoom<f16> = 12;
+
 // Few rows: one workgroup walks a part of one key head's blocks for 16 or 32 rows (NT
 // tiles), its four waves taking every fourth block.  The operands come straight from
 // memory in the layout the products want (16 x 16 x 32 MFMAs, P in registers): lane
@@ -102,6 +108,9 @@ __device__ __forceinline__ int64_t lse_at(const CacheAttn& a, int b, int kvh, in
 // accumulators hold keys 16 G + 4 t + i of row gi, which is the order of the 16 bytes
 // that a lane reads of v8's row 16 dt + gi.  Keys and values of a wave's next block are
 // asked for as soon as those of this one are used.
+//
+// A block's P lie under its own maximum, and its product is added to O in fp32 under that
+// of the walk and with the block's value scale: O holds the values' own size.
 //
 // Bound by the cache's bytes: a token each of 8 requests over 168,716 tokens in all, 8 heads
 // of 128 (345 MB), takes 68 us with the join's 5, 5.1 TB/s (a copy of 1 GiB: 5.0); one over
@@ -201,7 +210,7 @@ void few_rows_kernel(CacheAttn a, Parts p) {
   for (; j < j1; j += 4) {
     const int jn = j + 4 < j1 ? j + 4 : j;  // past the end: this block again, unused
     const float c = a.scale_log2 * ks_next > 0x1p-126f ? a.scale_log2 * ks_next : 0x1p-126f;
-    const int ev = exponent_of(vs_next);
+    const float unit = pow2i(exponent_of(vs_next));
     f32x4 s[NT][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -219,8 +228,7 @@ void few_rows_kernel(CacheAttn a, Parts p) {
     for (int t = 0; t < 4; ++t) ask_k(jn, t);
     const bool part = 64 * j + 64 > all.least;  // some row sees the block in part
     vec8 pf[NT][2];
-    float down[NT];
-    const float fev = (float)ev;
+    float down[NT], up[NT];  // what is there, and what the block adds, to the new maximum
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       if (part) {
@@ -232,10 +240,12 @@ void few_rows_kernel(CacheAttn a, Parts p) {
       float mx = s[nt][0][0];
 #pragma unroll
       for (int x = 1; x < 16; ++x) mx = __builtin_elementwise_maximum(mx, s[nt][x / 4][x % 4]);
-      const float m_new = __builtin_elementwise_maximum(m[nt], __builtin_fmaf(max_quarters(mx), c, fev));
+      const float top = max_quarters(mx) * c;  // the block's own, under which its P lie
+      const float m_new = __builtin_elementwise_maximum(m[nt], top);
       const float base = m_new == kNegInf ? 0.0f : m_new;
       down[nt] = fast_exp2(m[nt] - base);
-      const float off = fev - base;
+      up[nt] = fast_exp2(top - base) * pow2i(-kRoom<T>);
+      const float off = (float)kRoom<T> - (top == kNegInf ? 0.0f : top);
       float sum = 0.0f;
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
@@ -243,7 +253,8 @@ void few_rows_kernel(CacheAttn a, Parts p) {
         sum += e;
         pf[nt][x / 8][x % 8] = from_f32<T>(e);
       }
-      l[nt] = __builtin_fmaf(l[nt], down[nt], sum * pow2i(-ev));
+      l[nt] = __builtin_fmaf(l[nt], down[nt], sum * up[nt]);
+      up[nt] *= unit;
       m[nt] = m_new;
     }
     // NaN bytes of a block that some row sees in part count for the rows that see them alone.
@@ -287,10 +298,11 @@ void few_rows_kernel(CacheAttn a, Parts p) {
       const vec8 v0 = From8<T>::cvt(vw[dt][0], vw[dt][1]), v1 = From8<T>::cvt(vw[dt][2], vw[dt][3]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        f32x4 t = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        t = Mfma<T>::mma(v0, pf[nt][0], t);
+        t = Mfma<T>::mma(v1, pf[nt][1], t);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[nt][dt][i] *= down[nt];
-        o[nt][dt] = Mfma<T>::mma(v0, pf[nt][0], o[nt][dt]);
-        o[nt][dt] = Mfma<T>::mma(v1, pf[nt][1], o[nt][dt]);
+        for (int i = 0; i < 4; ++i) o[nt][dt][i] = __builtin_fmaf(o[nt][dt][i], down[nt], t[i] * up[nt]);
       }
       ask_v(jn, dt);
     }
@@ -472,10 +484,18 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 // chunk c of row r at c ^ swz(r), so that the 16 rows that a lane group reads at once
 // lie in different banks.
 //
-// A row's offset m is the maximum of its first half block, and later halves need no
-// maximum; their P' may pass 1.  Where a half's sum passes a bound (2^15 in fp16, whose
-// range ends there; 2^40 in bf16), or is NaN, the workgroup walks again with the rows'
-// exact maxima.  (Rescaling O inside the walk costs it 60 registers: 4310 us, below 3600.)
+// Here the value scale 2^ev is added to the exponent,
+//   P' = exp2(u + ev - m),  O = sum P' v8,  l = sum 2^(least - ev) P',  least the least ev,
+// so that O holds the true sum over 2^m and l the softmax's denominator over 2^(m - least).
+// A row's offset m comes from its first half block, and later halves need no maximum: in
+// bf16 that of u + ev, in fp16 that of u plus least, so that P' is no less than a token's
+// weight against the half's heaviest.  Where a half's sum passes a bound (fp16's largest
+// number; 2^40 in bf16), or is NaN, or the half's scores are all -inf, or the value scales
+// are more than 2^kSpread apart, the workgroup walks with care: band by band of scales so
+// close, each walked once for the rows' maxima of u + ev and once for its products, and O
+// and l brought from band to band.  The next band's offset lies no more than kFar below the
+// largest so far, which leaves O room in fp32.  (Rescaling O inside the walk costs it 60
+// registers: 4310 us, below 3600.)
 //
 // Bound by instructions: a block costs a wave 64 MFMAs (1024 cycles), 32 exponentials with
 // their sums and 128 conversions of bytes, about 2350 cycles with the MFMAs beside them.
@@ -495,12 +515,37 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 template <typename T>
 constexpr float kMaxSum = 0x1p40f;
 template <>
-constexpr float kMaxSum<f16> = 0x1p15f;
+constexpr float kMaxSum<f16> = 65504.0f;
+template <typename T>
+constexpr int kSpread = 32;
+template <>
+constexpr int kSpread<f16> = 8;
+constexpr float kFar = 80.0f;
 
 template <typename T>
 constexpr bool kIsBf16 = false;
 template <>
 constexpr bool kIsBf16<bf16> = true;
+
+// Of blocks j0 .. j1 - 1: the largest exponent of a value scale below `below`, and the
+// least one; without any, one below and one above the range.
+struct Span {
+  int top, least;
+};
+__device__ __forceinline__ Span span_of(const float* vsc, int j0, int j1, int below) {
+  Span s = {-kMaxScaleExp - 1, kMaxScaleExp + 1};
+  for (int j = j0 + threadIdx.x % 64; j < j1; j += 64) {
+    const int e = exponent_of(vsc[j]);
+    s.top = e < below && e > s.top ? e : s.top;
+    s.least = e < s.least ? e : s.least;
+  }
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_xor(s.top, o), l = __shfl_xor(s.least, o);
+    s.top = t > s.top ? t : s.top;
+    s.least = l < s.least ? l : s.least;
+  }
+  return {uniform_i32(s.top), uniform_i32(s.least)};
+}
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 constexpr int kSmall = 4;
 
@@ -550,6 +595,7 @@ void many_rows_kernel(CacheAttn a, Parts p) {
   const int j0 = split * p.per;
   const int j1 = j0 + p.per < nblk ? j0 + p.per : nblk;
   if (split > 0 && j0 >= nblk) return;  // the first part of a tile always answers
+  const Span span = span_of(a.c.v_scale + (int64_t)bh * a.c.nb, j0, j1, kMaxScaleExp + 1);
   const Reach mine = reach(a, n, kRows * tile + 32 * wave, kRows * tile + 32 * wave + 32);
   const int own = uniform_i32(mine.most), least = uniform_i32(mine.least);
 
@@ -745,20 +791,30 @@ void many_rows_kernel(CacheAttn a, Parts p) {
       if (__ballot(bad != 0)) nan_found = true;
     };
 
-    bool dirty = false, exact = false;
-    auto block = [&](int j, int slot, auto kind) {
+    auto value_exponent = [&](int j) {
+      return exponent_of(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs64), j & 63)));
+    };
+    bool dirty = false;
+    // kCareful: the offsets are known; every block counts as one that rows see in part.
+    auto block = [&](int j, int slot, int e, auto kind, auto how) {
       constexpr bool part = decltype(kind)::value;  // some row of the wave sees the block in part
+      constexpr bool careful = decltype(how)::value;
       const uint8_t* tile8 = ring + slot * kSlot;
-      const float c = key_scale(j);
-      const int e = exponent_of(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs64), j & 63)));
-      const float ev = (float)e, unit = pow2i(-e);
+      const float c = key_scale(j), ev = (float)e, unit = pow2i(span.least - e);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         qk(tile8, h);
         if constexpr (part) mask(j, h);
-        if (h == 0 && j == j0 && !exact) raise(h, c, ev);
+        if constexpr (!careful) {
+          if (h == 0 && j == j0) {
+            raise(h, c, kIsBf16<T> ? ev : (float)span.least);
+            if (__ballot((m[0] == kNegInf && vis[0] > 64 * j0) || (m[1] == kNegInf && vis[1] > 64 * j0))) dirty = true;
+          }
+        }
         exps(h, c, ev);
-        if (__ballot(!(sum[0] <= kMaxSum<T> && sum[1] <= kMaxSum<T>))) dirty = true;
+        if constexpr (!careful) {
+          if (__ballot(!(sum[0] <= kMaxSum<T> && sum[1] <= kMaxSum<T>))) dirty = true;
+        }
         l[0] = __builtin_fmaf(sum[0], unit, l[0]);
         l[1] = __builtin_fmaf(sum[1], unit, l[1]);
         if constexpr (part) pv_part(tile8, h);
@@ -766,7 +822,7 @@ void many_rows_kernel(CacheAttn a, Parts p) {
       }
     };
     // Blocks before `whole` are seen whole by every row of the wave that sees any token.
-    const int whole = own == 0 ? 0 : least / 64 < j1 ? least / 64 : j1;
+    int whole = own == 0 ? 0 : least / 64 < j1 ? least / 64 : j1;
     int j, slot;
     auto begin = [&] {
       j = j0, slot = 0;
@@ -781,44 +837,79 @@ void many_rows_kernel(CacheAttn a, Parts p) {
       if ((j & 63) == 0 && j > j0) scales(j);
       if (j + 2 < j1) fetch(j + 2, slot == 0 ? 2 : slot - 1);
     };
-    m[0] = m[1] = kNegInf;
-    for (;;) {
+    auto clear = [&] {
+      m[0] = m[1] = kNegInf;
       l[0] = l[1] = 0.0f;
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
         for (int qt = 0; qt < 2; ++qt) o[dt][qt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      if (j0 >= j1) break;
+    };
+    clear();
+    bool careful = span.top - span.least > kSpread<T>;  // workgroup-uniform
+    if (!careful && j0 < j1) {
       begin();
       for (; j < whole; ++j) {
         next();
-        block(j, slot, Flag<false>{});
+        block(j, slot, value_exponent(j), Flag<false>{}, Flag<false>{});
         slot = slot == 2 ? 0 : slot + 1;
       }
       for (; j < j1; ++j) {
         next();
-        if (64 * j < own) block(j, slot, Flag<true>{});
+        if (64 * j < own) block(j, slot, value_exponent(j), Flag<true>{}, Flag<false>{});
         slot = slot == 2 ? 0 : slot + 1;
       }
       if (lane == 0) wave_dirty[wave] = dirty ? 1 : 0;
       __syncthreads();  // the ring is free, the flags are there
-      if (exact || !(wave_dirty[0] | wave_dirty[1] | wave_dirty[2] | wave_dirty[3])) break;  // workgroup-uniform
-      exact = true;
-      begin();
-      for (; j < j1; ++j, slot = slot == 2 ? 0 : slot + 1) {  // the rows' maxima
-        next();
-        if (64 * j >= own) continue;
-        const float c = key_scale(j);
-        const float ev = (float)exponent_of(
-            __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs64), j & 63)));
+      careful = uniform_i32(wave_dirty[0] | wave_dirty[1] | wave_dirty[2] | wave_dirty[3]) != 0;
+      if (careful) clear();
+    }
+    if (careful) {
+      whole = j0;
+      float reached[2] = {kNegInf, kNegInf};  // the largest u + ev so far
+      for (int band = span.top;;) {           // value scales of kSpread exponents up to `band`
+        auto mine = [&](int j, int e) { return 64 * j < own && e <= band && e >= band - kSpread<T>; };
+        const float held[2] = {m[0], m[1]};
+        m[0] = m[1] = kNegInf;
+        begin();
+        for (; j < j1; ++j, slot = slot == 2 ? 0 : slot + 1) {  // the rows' maxima
+          next();
+          const int e = value_exponent(j);
+          if (!mine(j, e)) continue;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          qk(ring + slot * kSlot, h);
-          if (j >= whole) mask(j, h);
-          raise(h, c, ev);
+          for (int h = 0; h < 2; ++h) {
+            qk(ring + slot * kSlot, h);
+            mask(j, h);
+            raise(h, key_scale(j), (float)e);
+          }
         }
+        __syncthreads();  // the ring is free
+#pragma unroll
+        for (int qt = 0; qt < 2; ++qt) {
+          float f = 1.0f;
+          if (m[qt] == kNegInf) {  // nothing of the band, or nothing that counts
+            m[qt] = held[qt];
+          } else {
+            reached[qt] = __builtin_elementwise_maximum(reached[qt], m[qt]);
+            m[qt] = __builtin_elementwise_maximum(m[qt], reached[qt] - kFar) - (float)kRoom<T>;
+            if (held[qt] != kNegInf) f = fast_exp2(held[qt] - m[qt]);
+          }
+          l[qt] *= f;
+#pragma unroll
+          for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[dt][qt][i] *= f;
+        }
+        begin();
+        for (; j < j1; ++j, slot = slot == 2 ? 0 : slot + 1) {
+          next();
+          const int e = value_exponent(j);
+          if (mine(j, e)) block(j, slot, e, Flag<true>{}, Flag<true>{});
+        }
+        band = span_of(vsc, j0, j1, band - kSpread<T>).top;
+        if (band < span.least) break;
+        __syncthreads();  // the ring is free
       }
-      __syncthreads();
     }
     if (nan_found) {  // wave-uniform, rare: rows that see a NaN among the values get one
       for (int j = whole > j0 ? whole : j0; j < j1 && 64 * j < own; ++j) {
@@ -849,17 +940,18 @@ void many_rows_kernel(CacheAttn a, Parts p) {
     }
     __syncthreads();  // the ring is free
 
-    if (nblk > p.per) {
+    const float size = pow2i(span.least);
+    if (nblk > p.per) {  // under the offset of l, as few_rows_kernel's
       const int64_t part = part_at(a, p, split * a.c.B + b, kvh, 8 * tile + 2 * wave);
 #pragma unroll
       for (int qt = 0; qt < 2; ++qt) {
         float* po = p.o + (part + qt) * (16 * D) + gi * D + 4 * G;
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt) = o[dt][qt];
+        for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt) = o[dt][qt] * size;
         const float all = sum_quarters(l[qt]);
         if (G == 0) {
           float* ml = p.ml + (part + qt) * 32 + 2 * gi;
-          ml[0] = vis[qt] > 64 * j0 ? m[qt] : kNegInf;  // a row that saw none of this part
+          ml[0] = vis[qt] > 64 * j0 ? m[qt] - (float)span.least : kNegInf;  // a row that saw none of this part
           ml[1] = vis[qt] > 64 * j0 ? all : 0.0f;
         }
       }
@@ -869,7 +961,7 @@ void many_rows_kernel(CacheAttn a, Parts p) {
     for (int qt = 0; qt < 2; ++qt) {
       const float all = sum_quarters(l[qt]);
       const bool empty = vis[qt] == 0 || all == 0.0f;
-      const float inv = 1.0f / all;
+      const float inv = size / all;
       const int row = 32 * wave + 16 * qt + gi;
       uint8_t* orow = ring + row * (2 * D);
       const int swz = (row / (128 / D)) % (D / 8);
@@ -884,7 +976,7 @@ void many_rows_kernel(CacheAttn a, Parts p) {
       }
       const int r = kRows * tile + row;
       if (a.lse && G == 0 && r < rows)
-        a.lse[lse_at(a, b, kvh, r)] = empty ? kNegInf : (m[qt] + __builtin_log2f(all)) * kLn2;
+        a.lse[lse_at(a, b, kvh, r)] = empty ? kNegInf : (m[qt] - (float)span.least + __builtin_log2f(all)) * kLn2;
     }
     __syncthreads();
 #pragma unroll

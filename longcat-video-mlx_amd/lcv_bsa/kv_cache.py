@@ -240,8 +240,10 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
     count as that long); it shapes the launch of many rows, so a close one serves
     short histories in a long cache.
 
-    Sums are fp32.  Where the scales of the values that a row sees are 2^x apart, a
-    token whose weight is below 2^(x - 126) may be left out of the row's sum.
+    Sums are fp32.  Before they meet the values, probabilities are rounded to q's type
+    once: by half a step of it, in fp16 by up to 2^-25 of the row's largest, however far
+    apart the blocks' scales are.  A token whose weight is below 2^-40 of the heaviest's
+    may be left out of the row's sum.
 
     Returns ``out`` ``[B, Hq, S, D]`` in q's dtype, or ``(out, lse)`` with the fp32
     ``[B, Hq, S]`` log of each row's sum (-inf where nothing is seen)."""

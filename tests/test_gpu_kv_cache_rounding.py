@@ -1,0 +1,107 @@
+"""What the attention over an 8-bit cache may lose to rounding, judged number by number:
+value scales far apart, channels that only some blocks fill."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import cache_reference as R
+from test_gpu_kv_cache import BF16, F16, _gen, _rows, _within
+
+pytestmark = pytest.mark.gpu
+
+
+def _head(c, h):
+    from lcv_bsa import KVCache8
+
+    return KVCache8(*(t[:, h:h + 1].clone(memory_format=torch.contiguous_format) for t in (c.k8, c.v8, c.k_scale, c.v_scale)))
+
+
+def _judge(q, c, lengths, out, lse, sm_scale=None):
+    """Each channel by what its own values carry: P is rounded to q's type once (half a step
+    u of each; in fp16 no less than 2^-25 of the row's largest, below which it is
+    subnormal), the output once, and the scores' fp32 sums as R.attention has them."""
+    want, want_lse, _, tol_lse, probs, tol_p = R.attention(q, c, lengths, sm_scale=sm_scale)
+    v = R.values(c)[1].abs()
+    u = torch.finfo(q.dtype).eps / 2
+    size = probs @ v
+    tol = u * size + u * want.abs() + tol_p[..., None] * size
+    if q.dtype == F16:
+        tol += 2.0 ** -25 * probs.amax(-1, keepdim=True) * v[:, :, :lengths[0]].sum(2, keepdim=True)
+    _within(out, want, tol + (2.0 ** -25 if q.dtype == F16 else 2.0 ** -134))
+    _within(lse, want_lse, tol_lse)
+
+
+def _values(kind, gen, device, H, n, D):
+    """[1, H, n, D] fp32, and the type of the queries."""
+    v = torch.randn(1, H, n, D, generator=gen, device=device)
+    j = torch.arange(n, device=device) // 64
+    if kind in ("outlier, 2e-3", "late outlier, 2e-3", "outlier, 1e-4"):
+        v *= float(kind[-4:])
+        v[:, :, (10 if kind[0] == "o" else n - 70), 3] = 6e4  # its block's scale is 2^8: the rest there is zero
+        return v, F16
+    blocks = (n + 63) // 64
+    mine = torch.arange(D, device=device) % blocks == j[:, None]  # a channel is filled by one block of `blocks`
+    if kind == "steps":
+        return v * mine * torch.exp2(14.0 - 32.0 * j[:, None] / (blocks - 1)), F16
+    if kind == "rising steps":
+        return v * mine * torch.exp2(-18.0 + 32.0 * j[:, None] / (blocks - 1)), F16
+    assert kind in ("far", "far, rising")
+    e = 60.0 - 120.0 * j[:, None] / (blocks - 1)
+    return v * mine * torch.exp2(e if kind == "far" else -e), BF16
+
+
+KINDS = ["outlier, 2e-3", "late outlier, 2e-3", "outlier, 1e-4", "steps", "rising steps", "far", "far, rising"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("S", [1, 40, 200])
+@pytest.mark.parametrize("D", [64, 128])
+def test_value_scales_far_apart(device, kind, S, D):
+    from lcv_bsa import KVCache8, cache_append, cached_attention
+
+    gen = _gen(device, S + D)
+    n = 576
+    v, dtype = _values(kind, gen, device, 1, n, D)
+    k = torch.randn(1, 1, n, D, generator=gen, device=device)
+    c = cache_append(KVCache8.empty(1, 1, n, D, device), k, v, 0)
+    q = _rows(gen, device, 1, 1, S, D, dtype)
+    out, lse = cached_attention(q, c, n - 5, return_lse=True)
+    _judge(q, c, [n - 5], out, lse)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_value_scales_far_apart_in_whole_walks(device, kind, D):
+    """512 walks of two tiles each, which are not split."""
+    from lcv_bsa import KVCache8, cache_append, cached_attention
+
+    gen = _gen(device, D)
+    H, S, n = 512, 130, 1100
+    v, dtype = _values(kind, gen, device, H, n, D)
+    k = torch.randn(1, H, n, D, generator=gen, device=device)
+    c = cache_append(KVCache8.empty(1, H, n, D, device), k, v, 0)
+    q = _rows(gen, device, 1, H, S, D, dtype)
+    out, lse = cached_attention(q, c, n - 3, return_lse=True)
+    for h in (0, H - 1):
+        _judge(q[:, h:h + 1], _head(c, h), [n - 3], out[:, h:h + 1], lse[:, h:h + 1])
+
+
+@pytest.mark.parametrize("S", [1, 100])
+def test_scores_far_below_a_first_block_of_minus_infinity(device, S):
+    """The first block's products overflow to -inf; what is left has the whole weight,
+    however low its scores are."""
+    from lcv_bsa import KVCache8, cache_append, cached_attention
+
+    k = torch.zeros(1, 1, 128, 64, device=device)
+    k[:, :, :64, 0] = -1.0  # stored as -256
+    k[:, :, 64:, 1] = 1.0
+    c = cache_append(KVCache8.empty(1, 1, 128, 64, device), k, torch.ones_like(k), 0)
+    q = torch.zeros(1, 1, S, 64, dtype=BF16, device=device)
+    q[..., 0], q[..., 1] = 2.0 ** 120, -4096.0
+    out, lse = cached_attention(q, c, 128, return_lse=True)
+    assert bool((out == 1).all())
+    assert float((lse - (math.log(64) - 512)).abs().max()) <= 2.0 ** -13  # fp32 near 2^9: 2^-15 a rounding
