@@ -506,10 +506,12 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 // kBytes (bf16, D = 128, long walks): the keys' bytes go to 16 x 16 x 128 MFMAs as they are,
 // and a row's values as the sum of two e4m3 numbers under the row's 2^e and 2^(e - 4): two
 // passes at twice bf16's rate, and 64 conversions less.  e4m3's 4 bits twice are bf16's 8,
-// so that values of 2^-14.8 of the row's largest and more are exact, and those below within
-// 2^-22 of the largest.  Where more than kSmall of a lane's 64 values are not held to 2^-12
-// of themselves (a row whose largest is far above the rest, which its keys may not answer;
-// normally distributed rows have 0.1 a lane), the workgroup converts the keys instead.
+// so that values from 2^(e - 6) on (2^-14.8 of the row's largest) are exact; one below is
+// off by no more than 2^(e - 14), nor than itself.  What that adds up to in a score, if
+// every key held its scale's largest number there, has to stay below kLost in u for all
+// rows of the workgroup (normed rows of 128 against normed keys: 2^-20 for each such value,
+// of which a row has 0.02), else it converts the keys: a row whose largest value is far
+// above the rest, which its keys may not answer, or an infinite one.
 // 12,480 queries of 32 heads over 18,720 tokens then take 3376 us, 1134 TFLOP/s, against
 // 3637 (a product of 8192^3 makes 1214); 2048 over 2048 of 32 heads 75 against 78.
 template <typename T>
@@ -526,6 +528,14 @@ template <typename T>
 constexpr bool kIsBf16 = false;
 template <>
 constexpr bool kIsBf16<bf16> = true;
+
+// The largest key scale of blocks j0 .. j1 - 1.
+__device__ __forceinline__ float largest_scale(const float* ksc, int j0, int j1) {
+  float most = 0.0f;
+  for (int j = j0 + threadIdx.x % 64; j < j1; j += 64) most = fmaxf(most, ksc[j]);
+  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+  return most;
+}
 
 // Of blocks j0 .. j1 - 1: the largest exponent of a value scale below `below`, and the
 // least one; without any, one below and one above the range.
@@ -547,7 +557,7 @@ __device__ __forceinline__ Span span_of(const float* vsc, int j0, int j1, int be
   return {uniform_i32(s.top), uniform_i32(s.least)};
 }
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-constexpr int kSmall = 4;
+constexpr float kLost = 0x1p-14f;
 
 // The least e >= -123 with |q| <= 448 2^e = 1.75 2^(e + 8) in the lane's row, of which it
 // holds a quarter.
@@ -989,17 +999,21 @@ void many_rows_kernel(CacheAttn a, Parts p) {
     }
   };
   if constexpr (kBytes) {
-    int small = 0;  // of the lane's 64 values, those not held to 2^-12 of themselves
+    const float answer = 448.0f * a.scale_log2 * largest_scale(a.c.k_scale + (int64_t)bh * a.c.nb, j0, j1);
+    bool fine = true;
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
-      const float bound = 0.25f * pow2i(byte_exponent<D>(qf[qt]));
+      const float unit = pow2i(byte_exponent<D>(qf[qt]));
+      float lost = 0.0f;
 #pragma unroll
       for (int x = 0; x < D / 4; ++x) {
         const float y = __builtin_fabsf(to_f32(qf[qt][x / 8][x % 8]));
-        small += y != 0.0f && y < bound ? 1 : 0;
+        if (y < 0x1p-6f * unit) lost += fminf(y, 0x1p-14f * unit);
+        if (y == __builtin_inff()) lost = y;
       }
+      fine = fine && sum_quarters(lost) * answer <= kLost;  // false for a NaN
     }
-    if (!__syncthreads_or(small > kSmall)) {
+    if (!__syncthreads_or(!fine)) {
       rest(Flag<true>{});
       return;
     }

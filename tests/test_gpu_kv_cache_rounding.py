@@ -1,5 +1,6 @@
 """What the attention over an 8-bit cache may lose to rounding, judged number by number:
-value scales far apart, channels that only some blocks fill."""
+value scales far apart, channels that only some blocks fill, queries beside large values
+that no key answers."""
 
 from __future__ import annotations
 
@@ -105,3 +106,41 @@ def test_scores_far_below_a_first_block_of_minus_infinity(device, S):
     out, lse = cached_attention(q, c, 128, return_lse=True)
     assert bool((out == 1).all())
     assert float((lse - (math.log(64) - 512)).abs().max()) <= 2.0 ** -13  # fp32 near 2^9: 2^-15 a rounding
+
+
+@pytest.mark.parametrize("scale", [128 ** -0.5, 1.0])
+def test_sparse_queries_beside_an_unanswered_value(device, scale):
+    """Walks of 32 blocks in bf16, D = 128: rows of one large value in a channel where keys
+    are zero and two small ones in each quarter, which are all that the scores hold."""
+    from lcv_bsa import KVCache8, cache_append, cached_attention
+
+    gen = _gen(device, 9)
+    H, S, D, n = 512, 130, 128, 1999
+    k, v = (torch.randn(1, H, 2048, D, generator=gen, device=device) for _ in range(2))
+    k[..., 5] = 0.0
+    at = torch.tensor([3, 20, 35, 60, 70, 90, 100, 127], device=device)
+    q = torch.zeros(1, H, S, D, device=device)
+    q[..., at] = torch.randn(1, H, S, len(at), generator=gen, device=device) * 2
+    sizes = [12, 16, 20, 22, 24, 30, 100]
+    for i, e in enumerate(sizes):
+        q[:, i::len(sizes), :, 5] = 2.0 ** e
+    c = cache_append(KVCache8.empty(1, H, 2048, D, device), k, v, 0)
+    q = q.to(BF16)
+    out, lse = cached_attention(q, c, n, sm_scale=scale, return_lse=True)
+    for h in range(len(sizes)):
+        _judge(q[:, h:h + 1], _head(c, h), [n], out[:, h:h + 1], lse[:, h:h + 1], scale)
+
+
+def test_an_infinite_query_over_a_long_walk(device):
+    """A row whose only value is infinite and whose scores are all -inf sees nothing."""
+    from lcv_bsa import KVCache8, cache_append, cached_attention
+
+    gen = _gen(device, 2)
+    H, S, D = 512, 130, 128
+    k, v = (torch.randn(1, H, 2048, D, generator=gen, device=device) for _ in range(2))
+    k[..., 5] = -1.0
+    c = cache_append(KVCache8.empty(1, H, 2048, D, device), k, v, 0)
+    q = torch.zeros(1, H, S, D, dtype=BF16, device=device)
+    q[..., 5] = math.inf
+    out, lse = cached_attention(q, c, 2000, return_lse=True)
+    assert not out.any() and bool((lse == -math.inf).all())
