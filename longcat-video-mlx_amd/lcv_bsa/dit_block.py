@@ -205,8 +205,7 @@ class Attention(nn.Module, BSAAttention):
         q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
         o = torch.empty((B, N, H, D), dtype=x.dtype, device=x.device)
         eight = return_kv and self.kv_cache_8bit
-        if (self.enable_bsa and shape is not None
-                and (not return_kv or eight or self._cache_fusible(qkv))):
+        if self.enable_bsa and shape is not None and (not return_kv or self._cache_fusible(qkv)):
             validate_backend(self.bsa_backend)
             geom = bsa_geometry(shape, self.bsa_chunk_thw, self.bsa_shape_policy)
             if geom is not None:
