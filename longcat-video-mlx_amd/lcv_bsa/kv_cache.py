@@ -24,6 +24,7 @@ import math
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .block_sparse_attention import _dtype_code, _require_device
@@ -163,6 +164,8 @@ def _no_grad(what: str, *ts: torch.Tensor) -> None:
     for t in ts:
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ValueError(f"{what} has no forward-mode derivative: call it on detached tensors")
 
 
 def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start: Ints,

@@ -16,6 +16,7 @@ import functools
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .block_sparse_attention import _dtype_code, _require_device, _stream
@@ -127,18 +128,29 @@ def _rotate(x: torch.Tensor, positions: torch.Tensor, dims: Optional[tuple], bas
     return out
 
 
+def _watched(x: torch.Tensor) -> bool:
+    """A derivative of what becomes of ``x`` may be wanted, in reverse or in forward mode."""
+    return (x.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0
+
+
 class _RopeNd(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, positions, dims, base, inverse):
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.how = dims, base, inverse
         return _rotate(x, positions, dims, base, inverse)
 
     @staticmethod
     def backward(ctx, g):
         dims, base, inverse = ctx.how
-        turn = _RopeNd.apply if torch.is_grad_enabled() else _rotate  # a second derivative is wanted, or not
+        turn = _RopeNd.apply if torch.is_grad_enabled() or _watched(g) else _rotate  # a further derivative is wanted, or not
         return turn(g, *ctx.saved_tensors, dims, base, not inverse), None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, t, *_):
+        turn = _RopeNd.apply if t.requires_grad and torch.is_grad_enabled() else _rotate
+        return turn(t, *ctx.saved_tensors, *ctx.how)
 
 
 def rope_nd(x: torch.Tensor, positions: torch.Tensor, dims: Optional[Sequence[int]] = None, *,
@@ -149,7 +161,8 @@ def rope_nd(x: torch.Tensor, positions: torch.Tensor, dims: Optional[Sequence[in
 
     ``dims``: the even number of dims that each axis turns, summing to D; by
     default the t / h / w split of ``rope_dims`` for three axes, else equal
-    parts.  Differentiable in ``x`` (as often as wanted); positions get no gradient.
+    parts.  Differentiable in ``x`` (as often as wanted, and in forward mode);
+    positions get no gradient.
     A backward pass that is captured into a graph takes its gradients with
     ``torch.autograd.grad``, while no graph of the same leaves that was made outside
     of the capture is alive: torch would have to order the two streams there."""
@@ -157,6 +170,6 @@ def rope_nd(x: torch.Tensor, positions: torch.Tensor, dims: Optional[Sequence[in
     dims = None if dims is None else tuple(dims)
     if positions.requires_grad:
         positions = positions.detach()
-    if x.requires_grad and torch.is_grad_enabled():
+    if _watched(x):
         return _RopeNd.apply(x, positions, dims, float(base), False)
     return _rotate(x, positions, dims, float(base), False)

@@ -265,3 +265,27 @@ def test_c_entries_refuse_overlaps():
     other = _lib.Strides(8192, 64, 128)
     assert lib.lcv_bsa_rope_nd(fake, 1, 1, 2, 4, 64, st, fake, 0, 0, 1, (ctypes.c_int64 * 1)(64), 1, 1e4, 0, fake, other, None) == _lib.ERR_LAYOUT
     assert b"in place" in lib.lcv_bsa_last_error()
+
+
+def test_tangents_are_refused(on_cpu):
+    """Forward-mode derivatives are not dropped; without a tangent the calls go on."""
+    from torch.autograd import forward_ad
+
+    from lcv_bsa import attention_weights, cache_append, cache_evict, cached_attention
+
+    c, q, w = _cache(), torch.zeros(2, 4, 3, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 128)
+    x, lse = torch.zeros(2, 2, 3, 64), torch.zeros(2, 4, 3)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda f: cache_append(c, f(x), x, 0), lambda f: cache_append(c, x, f(x), 0),
+                     lambda f: cached_attention(f(q), c, 5), lambda f: cached_attention(q, c, 5, out=f(q.clone())),
+                     lambda f: attention_weights(f(q), c, 5, lse), lambda f: attention_weights(q, c, 5, f(lse)),
+                     lambda f: attention_weights(q, c, 5, lse, weights=f(w)), lambda f: cache_evict(c, 5, f(w), 10)):
+            with pytest.raises(ValueError, match="derivative"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(ValueError, match="derivative"):
+                call(dual)
+            with pytest.raises(AssertionError, match="reached"):
+                call(lambda t: dual(t).detach())

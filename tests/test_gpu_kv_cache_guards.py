@@ -1,12 +1,14 @@
-"""The 8-bit cache beside what watches or changes a layer: norms of other kinds."""
+"""The 8-bit cache beside what watches or changes a layer: norms of other kinds, forward-mode
+derivatives."""
 
 from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from conftest import NORM_CHANGES, changed_norms
-from test_gpu_kv_cache import BF16, _gen, _stored
+from test_gpu_kv_cache import BF16, F32, _gen, _stored
 from test_gpu_kv_cache_layer import _layer
 
 pytestmark = pytest.mark.gpu
@@ -54,3 +56,45 @@ def test_norms_of_different_eps(device):
     (out, plain), (out8, cache) = _both(m, x)
     assert torch.equal(out8, out)
     _same_keys(cache, plain)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rope_forward_mode(device, dtype):
+    """Linear in x: the tangent is turned as x is, to the bit; through a backward pass too."""
+    from lcv_bsa import rope_nd
+
+    gen = _gen(device, 1)
+    x, t, g = (torch.randn(1, 3, 20, 64, generator=gen, device=device).to(dtype) for _ in range(3))
+    pos = torch.randint(0, 90, (20, 3), generator=gen, device=device)
+    want, turned = rope_nd(x, pos), rope_nd(t, pos)
+    for leaf in (x, x.clone().requires_grad_(True)):
+        with forward_ad.dual_level():
+            y, dy = forward_ad.unpack_dual(rope_nd(forward_ad.make_dual(leaf, t), pos))
+            assert torch.equal(y, want) and torch.equal(dy, turned)
+    with forward_ad.dual_level():  # a tangent that is differentiated in its turn
+        r = t.clone().requires_grad_(True)
+        dy = forward_ad.unpack_dual(rope_nd(forward_ad.make_dual(x, r), pos)).tangent
+        (dr,) = torch.autograd.grad(dy, r, g)
+    z = x.clone().requires_grad_(True)
+    assert torch.equal(dr, torch.autograd.grad(rope_nd(z, pos), z, g)[0])
+    with forward_ad.dual_level():  # no tangent, none made
+        assert forward_ad.unpack_dual(rope_nd(x, pos)).tangent is None
+        z = x.clone().requires_grad_(True)
+        (dx,) = torch.autograd.grad(rope_nd(z, pos), z, forward_ad.make_dual(g, t))
+        back, dback = forward_ad.unpack_dual(dx)
+    z = x.clone().requires_grad_(True)
+    grads = [torch.autograd.grad(rope_nd(z, pos), z, h)[0] for h in (g, t)]
+    assert torch.equal(back, grads[0]) and torch.equal(dback, grads[1])
+
+
+def test_layer_forward_mode(device):
+    """A tangent is refused, not lost: where the cache is made and where it is read."""
+    m, x = _layer(device), _input(device)
+    more = torch.randn(1, 192, 256, generator=_gen(device, 4), device=device).to(BF16)
+    with torch.no_grad():
+        _, cache = m(x, GRID, return_kv=True)
+        with forward_ad.dual_level():
+            with pytest.raises(ValueError, match="derivative"):
+                m(forward_ad.make_dual(x, x), GRID, return_kv=True)
+            with pytest.raises(ValueError, match="derivative"):
+                m.forward_with_kv_cache(forward_ad.make_dual(more, more), (3, 8, 8), 2, cache)
