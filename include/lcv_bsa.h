@@ -498,7 +498,8 @@ typedef struct lcv_bsa_cache8 {
  * before start[b]; those are rounded again if it grows.  Rounding is to nearest,
  * ties to even; infinities, NaN and what lies beyond the scales' range become NaN.
  * Rows past the capacity, and items with a negative start, are left out; bytes
- * behind the last new row stay as they were.  start and counts are read on the
+ * behind the last new row stay as they were, those of its block under the block's
+ * new scale: tokens that stood there are lost.  start and counts are read on the
  * device.
  */
 int lcv_bsa_cache_append(lcv_bsa_cache8 c, const void* k, const void* v,

@@ -178,8 +178,10 @@ def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start: Ints,
     new rows within 448, and no less than it was where the block keeps rows before
     ``start`` (those are rounded again if it grows).  To nearest, ties to even;
     infinities, NaN and magnitudes over 448 * 2^60 become NaN.  Rows that would pass
-    the capacity and items with a negative start are left out; what stood behind
-    the last new row stays.  Returns the cache."""
+    the capacity and items with a negative start are left out.  Behind the last new
+    row the bytes stay, but in its block they stand under the new scale: tokens that
+    stood there are lost, so rows are written behind all that is to be kept, or
+    instead of it.  Returns the cache."""
     _require_device(cache.k8, k, v)
     _no_grad("cache_append", k, v)
     B, H, n, D = cache.shape
@@ -190,9 +192,10 @@ def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start: Ints,
     code = _dtype_code(k)
     if S > n:
         raise ValueError(f"{S} rows for a cache of {n} tokens")
+    rows = S if counts is None else 0 if isinstance(counts, torch.Tensor) else int(counts)  # that a plain start has to fit
     if counts is not None:
         counts = _ints(counts, "counts", B, cache.device, 0, S)
-    start = _ints(start, "start", B, cache.device, 0, n - S)
+    start = _ints(start, "start", B, cache.device, 0, n - rows)
     if S == 0:
         return cache
     k, ks = rows_of(k, "k")

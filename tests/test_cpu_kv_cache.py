@@ -289,3 +289,15 @@ def test_tangents_are_refused(on_cpu):
                 call(dual)
             with pytest.raises(AssertionError, match="reached"):
                 call(lambda t: dual(t).detach())
+
+
+def test_a_plain_start_has_to_fit_the_rows_counted(on_cpu):
+    from lcv_bsa import cache_append
+
+    c, x = _cache(), torch.zeros(2, 2, 10, 64)
+    for start, counts in ((126, 2), (128, 0), (128, _i(0, 0)), (121, _i(7, 3))):
+        with pytest.raises(AssertionError, match="reached"):
+            cache_append(c, x, x, start, counts)
+    for start, counts in ((127, 2), (129, 0), (129, _i(0, 0)), (-1, 2), (119, None)):
+        with pytest.raises(ValueError):
+            cache_append(c, x, x, start, counts)

@@ -1,5 +1,5 @@
 """The 8-bit cache beside what watches or changes a layer: norms of other kinds, forward-mode
-derivatives."""
+derivatives; appending near the capacity."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import torch
 from torch.autograd import forward_ad
 
 from conftest import NORM_CHANGES, changed_norms
-from test_gpu_kv_cache import BF16, F32, _gen, _stored
+from test_gpu_kv_cache import BF16, F32, _gen, _ints, _stored
 from test_gpu_kv_cache_layer import _layer
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +98,18 @@ def test_layer_forward_mode(device):
                 m(forward_ad.make_dual(x, x), GRID, return_kv=True)
             with pytest.raises(ValueError, match="derivative"):
                 m.forward_with_kv_cache(forward_ad.make_dual(more, more), (3, 8, 8), 2, cache)
+
+
+def test_append_near_the_capacity(device):
+    """A plain start stands for the same number in a tensor, also where the rows counted
+    alone fit."""
+    from lcv_bsa import KVCache8, cache_append
+
+    gen = _gen(device, 2)
+    x = torch.randn(2, 2, 10, 64, generator=gen, device=device)
+    for counts in (2, _ints(device, [2, 1])):
+        a, b = (KVCache8.empty(2, 2, 128, 64, device) for _ in range(2))
+        cache_append(a, x, x, 126, counts)
+        cache_append(b, x, x, _ints(device, [126, 126]), counts if torch.is_tensor(counts) else _ints(device, [2, 2]))
+        for (s, t), (u, w) in zip(_stored(a), _stored(b)):
+            assert torch.equal(s, u) and torch.equal(t, w) and bool(s[:, :, 126:127].any())
