@@ -27,7 +27,7 @@ import torch.nn.functional as F
 from .attention import BSAAttention, dense_attention, validate_backend
 from .block_ops import adaln_modulation, head_rms_norm, plain_tensors, residual_norm, swiglu, text_attention, unwatched
 from .block_sparse_attention import bsa_attention
-from .kv_cache import KVCache8, cache_append, cached_attention
+from .kv_cache import KVCache8, cache_append, cached_attention, no_derivative
 from .prepare import prepare_qk, prepare_qkv
 from .rope_3d import rope_3d, rope_dims
 from .rope_positions import grid_positions, rope_nd
@@ -205,6 +205,8 @@ class Attention(nn.Module, BSAAttention):
         q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
         o = torch.empty((B, N, H, D), dtype=x.dtype, device=x.device)
         eight = return_kv and self.kv_cache_8bit
+        if eight:
+            self._check_cache8(qkv)
         if self.enable_bsa and shape is not None and (not return_kv or self._cache_fusible(qkv)):
             validate_backend(self.bsa_backend)
             geom = bsa_geometry(shape, self.bsa_chunk_thw, self.bsa_shape_policy)
@@ -221,11 +223,12 @@ class Attention(nn.Module, BSAAttention):
                         self._split(qp, kp, v, shape, ncl, o)
                     else:
                         self._attend("all", qp, kp, v, shape, means=(qb, kb), out=o.transpose(1, 2))
+                except ValueError:
+                    self.last_indices, self.last_paths = {}, {}
+                else:
                     cache = self._cache8(kp, v) if eight else (kn, v) if return_kv else None
                     out = self.proj(o.view(B, N, C))
                     return (out, cache) if return_kv else out
-                except ValueError:
-                    self.last_indices, self.last_paths = {}, {}
         # The reference's sequence: norms, (cache,) RoPE, then BSA-or-dense.
         q, k = self.q_norm(q), self.k_norm(k)
         cache = (k, v)
@@ -245,6 +248,12 @@ class Attention(nn.Module, BSAAttention):
         return (plain_rms_norms(self.q_norm, self.k_norm) and self.q_norm.eps == self.k_norm.eps
                 and plain_tensors(*tensors, self.q_norm.weight, self.k_norm.weight))
 
+    def _check_cache8(self, qkv: torch.Tensor) -> None:
+        """Refuses what ``_cache8`` would, before any work goes into it."""
+        if self.head_dim not in (64, 128):
+            raise ValueError(f"an 8-bit cache holds head dims 64 and 128, got {self.head_dim}")
+        no_derivative("kv_cache_8bit", qkv, *self.k_norm.parameters())
+
     @staticmethod
     def _cache8(k: torch.Tensor, v: torch.Tensor) -> tuple[KVCache8, int]:
         """The 8-bit cache of rotated keys and values ``[B, H, N, D]``, and N."""
@@ -263,7 +272,7 @@ class Attention(nn.Module, BSAAttention):
             raise ValueError(f"an 8-bit cache {cache.shape} of {cached} tokens does not hold {ncl} frames of {Hl} x {Wl} "
                              f"before {N} new tokens of {B} items, {H} heads of {D}")
         q, k, v = (t.transpose(1, 2) for t in self.qkv(x).view(B, N, 3, H, D).unbind(2))
-        if D in (64, 128) and self._cache_fusible(q, k):
+        if self._cache_fusible(q, k):
             q, k = (head_rms_norm(t, m.weight, m.eps) for t, m in ((q, self.q_norm), (k, self.k_norm)))
         else:
             q, k = self.q_norm(q), self.k_norm(k)

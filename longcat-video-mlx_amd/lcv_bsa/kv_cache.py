@@ -160,7 +160,8 @@ def _ints(x: Ints, name: str, B: int, device: torch.device, lo: int, hi: int) ->
     return torch.full((B,), x, dtype=torch.int32, device=device)
 
 
-def _no_grad(what: str, *ts: torch.Tensor) -> None:
+def no_derivative(what: str, *ts: torch.Tensor) -> None:
+    """Raises for tensors that a gradient or a tangent goes through."""
     for t in ts:
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
@@ -183,7 +184,7 @@ def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start: Ints,
     stood there are lost, so rows are written behind all that is to be kept, or
     instead of it.  Returns the cache."""
     _require_device(cache.k8, k, v)
-    _no_grad("cache_append", k, v)
+    no_derivative("cache_append", k, v)
     B, H, n, D = cache.shape
     S = k.shape[2] if k.dim() == 4 else -1
     if k.shape != (B, H, S, D) or v.shape != (B, H, S, D) or k.dtype != v.dtype:
@@ -208,7 +209,7 @@ def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start: Ints,
 def _queries(what, q, cache, lengths, q_lens, sm_scale, max_len):
     """The arguments that attention and its weights share, checked."""
     _require_device(cache.k8, q)
-    _no_grad(what, q)
+    no_derivative(what, q)
     B, H, n, D = cache.shape
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D or q.shape[1] < H or q.shape[1] % H:
         raise ValueError(f"q must be [{B}, a multiple of {H}, S, {D}], got {tuple(q.shape)}")
@@ -259,7 +260,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
         out = q.new_empty((B, Hq, S, D))
     else:
         _require_device(q, out)
-        _no_grad("cached_attention", out)
+        no_derivative("cached_attention", out)
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
         if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
@@ -300,7 +301,7 @@ def attention_weights(q: torch.Tensor, cache: KVCache8, lengths: Ints, lse: torc
         if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float32):
             raise ValueError(f"{name} must be fp32 {shape}, got {t.dtype} {tuple(t.shape)}")
     _require_device(q, lse, *(t for t in (weights, out) if t is not None))
-    _no_grad("attention_weights", lse, *(t for t in (weights, out) if t is not None))
+    no_derivative("attention_weights", lse, *(t for t in (weights, out) if t is not None))
     if out is None:
         out = lse.new_empty(shape)
     elif not out.is_contiguous():
@@ -330,7 +331,7 @@ def cache_evict(cache: KVCache8, lengths: Ints, weights: torch.Tensor, keep: int
     behind the last), the kept tokens' weights (zeros behind), their old indices
     ``[B, H, keep]`` int32 (-1 behind) and the new lengths ``[B]`` int32."""
     _require_device(cache.k8, weights)
-    _no_grad("cache_evict", weights)
+    no_derivative("cache_evict", weights)
     B, H, n, D = cache.shape
     if tuple(weights.shape) != (B, H, n) or weights.dtype != torch.float32:
         raise ValueError(f"weights must be fp32 {(B, H, n)}, got {weights.dtype} {tuple(weights.shape)}")

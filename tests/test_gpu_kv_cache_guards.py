@@ -1,5 +1,5 @@
 """The 8-bit cache beside what watches or changes a layer: norms of other kinds, forward-mode
-derivatives; appending near the capacity."""
+derivatives; refusals before any work; appending near the capacity."""
 
 from __future__ import annotations
 
@@ -113,3 +113,21 @@ def test_append_near_the_capacity(device):
         cache_append(b, x, x, _ints(device, [126, 126]), counts if torch.is_tensor(counts) else _ints(device, [2, 2]))
         for (s, t), (u, w) in zip(_stored(a), _stored(b)):
             assert torch.equal(s, u) and torch.equal(t, w) and bool(s[:, :, 126:127].any())
+
+
+@pytest.mark.parametrize("bsa", [False, True])
+def test_refused_before_any_work(device, bsa, calls):
+    """A gradient through the cache, or a head dim that it does not hold."""
+    from lcv_bsa import dit_block
+
+    seen = [calls(dit_block, name) for name in ("prepare_qk", "prepare_qkv", "bsa_attention", "dense_attention", "rope_3d")]
+    m, x = _layer(device, bsa=bsa), _input(device)
+    with pytest.raises(ValueError, match="backward"):
+        m(x, GRID, return_kv=True)
+    small = _layer(device, heads=8, dim=32, bsa=bsa)
+    with torch.no_grad(), pytest.raises(ValueError, match="64 and 128"):
+        small(x, GRID, return_kv=True)
+    assert not any(seen)
+    with torch.no_grad():
+        m(x, GRID, return_kv=True)
+    assert any(seen)
