@@ -512,7 +512,8 @@ int lcv_bsa_cache_append(lcv_bsa_cache8 c, const void* k, const void* v,
  * head h reads key head h / (Hq / H)) over the first lengths[b] tokens of item b's
  * cache.  q_lens[b] (null: S) of its queries are real, and with `causal` set query
  * i sees the tokens up to lengths[b] - q_lens[b] + i: the real queries are the last
- * tokens.  out [B,Hq,S,D] and, if given, lse [B,Hq,S] (natural log of the sum of
+ * tokens.  out [B,Hq,S,D], which may be q itself, with q's strides, and does not
+ * overlap it otherwise, and, if given, lse [B,Hq,S] (natural log of the sum of
  * exp(sm_scale q.k)); rows that see no token get zeros and -inf.  max_len bounds
  * the lengths (longer ones count as max_len).  sm_scale >= 0; rows on 16-byte
  * boundaries.  lengths and q_lens are read on the device.  The workspace holds the

@@ -232,6 +232,47 @@ def _workspace(entry: str, Hq: int, S: int, B: int, H: int, n: int, D: int, max_
     return getattr(_lib.load(), entry)(Hq, S, _lib.Cache8(None, None, None, None, B, H, n, D), max_len)
 
 
+@functools.lru_cache(maxsize=1024)
+def _shared(shape: tuple, strides: tuple, apart: int) -> bool:
+    """Whether a tensor of this shape and these strides and one `apart` elements behind it
+    have an element in common; apart 0: whether it holds one element twice.  (A layout whose
+    dimensions are tangled beyond a few thousand steps of the search counts as one.)"""
+    dims = sorted(((st, n) for n, st in zip(shape, strides) if n > 1), reverse=True)
+    rest = [sum((n - 1) * st for st, n in dims[i:]) for i in range(len(dims) + 1)]
+    steps = 0
+
+    def search(i: int, left: int, moved: bool) -> bool:  # left = sum of d stride, |d| < n, from dims[i] on?
+        nonlocal steps
+        steps += 1
+        if steps > 4096:
+            return True
+        if abs(left) > rest[i]:
+            return False
+        if i == len(dims):
+            return moved
+        st, n = dims[i]
+        if st == 0:
+            return left == 0
+        lo, hi = -((rest[i + 1] - left) // st), (left + rest[i + 1]) // st
+        return any(search(i + 1, left - d * st, moved or d != 0) for d in range(max(lo, 1 - n), min(hi, n - 1) + 1))
+
+    return search(0, apart, apart != 0)
+
+
+def _apart(q: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether rows of ``out`` may be written while others of ``q`` (of its shape and dtype)
+    are read: it is q itself, or has no element of another row of it."""
+    size = q.element_size()
+    first, last = ((t.data_ptr(), t.data_ptr() + size * sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) for t in (q, out))
+    if first[1] < last[0] or last[1] < first[0]:
+        return True
+    strides = tuple(st for n, st in zip(q.shape, q.stride()) if n > 1)
+    if strides != tuple(st for n, st in zip(out.shape, out.stride()) if n > 1):
+        return False
+    apart, odd = divmod(last[0] - first[0], size)
+    return not odd and (apart == 0 or not _shared(tuple(n for n in q.shape if n > 1), strides, apart))
+
+
 def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens: Optional[Ints] = None,
                      causal: bool = False, sm_scale: Optional[float] = None, max_len: Optional[int] = None,
                      out: Optional[torch.Tensor] = None, return_lse: bool = False):
@@ -252,10 +293,12 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
     apart the blocks' scales are.  A token whose weight is below 2^-40 of the heaviest's
     may be left out of the row's sum.
 
-    Returns ``out`` ``[B, Hq, S, D]`` in q's dtype, or ``(out, lse)`` with the fp32
+    ``out`` may be q, or lie anywhere on its memory; its own elements lie apart.
+    Returns it (``[B, Hq, S, D]`` in q's dtype), or ``(out, lse)`` with the fp32
     ``[B, Hq, S]`` log of each row's sum (-inf where nothing is seen)."""
     lengths, q_lens, sm_scale, max_len = _queries("cached_attention", q, cache, lengths, q_lens, sm_scale, max_len)
     B, Hq, S, D = q.shape
+    given = out
     if out is None:
         out = q.new_empty((B, Hq, S, D))
     else:
@@ -263,7 +306,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
         no_derivative("cached_attention", out)
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError(f"out must be {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
-        if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+        if _shared(tuple(out.shape), out.stride(), 0):
             raise ValueError("out's elements share memory")
     lse = cache.k_scale.new_empty((B, Hq, S)) if return_lse else None
     if q.numel() == 0 or max_len == 0:
@@ -271,8 +314,9 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
         if return_lse:
             lse.fill_(-math.inf)
         return (out, lse) if return_lse else out
+    # A copy where out's rows cannot be written in place.
+    to, os = rows_of(out if given is None or _apart(q, given) else torch.empty_like(out, memory_format=torch.contiguous_format), "out")
     q, qs = rows_of(q, "q")
-    to, os = rows_of(out, "out")  # a copy where out's rows cannot be written in place
     size = _workspace("lcv_bsa_cached_attn_workspace_bytes", Hq, S, *cache.shape, max_len)
     ws = torch.empty((size,), dtype=torch.uint8, device=q.device) if size else None
     launch(q, "cached_attn", q.data_ptr(), _dtype_code(q), Hq, S, qs, cache._pointers(), lengths.data_ptr(),

@@ -301,3 +301,50 @@ def test_a_plain_start_has_to_fit_the_rows_counted(on_cpu):
     for start, counts in ((127, 2), (129, 0), (129, _i(0, 0)), (-1, 2), (119, None)):
         with pytest.raises(ValueError):
             cache_append(c, x, x, start, counts)
+
+
+def _addresses(shape, strides, first=0):
+    at = torch.tensor([first])
+    for n, st in zip(shape, strides):
+        at = (at[:, None] + torch.arange(n) * st).flatten()
+    return at.tolist()
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 4, 8), (1, 1, 5, 8), (2, 1, 1, 8), (3, 2, 2, 4)])
+def test_shared_elements(shape):
+    """Against the lists of addresses, for layouts of every kind."""
+    from lcv_bsa.kv_cache import _shared
+
+    layouts = [torch.empty(shape).stride(), torch.empty([shape[i] for i in (0, 2, 1, 3)]).transpose(1, 2).stride(),
+               (0, 64, 8, 1), (40, 16, 8, 1), (9, 3, 30, 1), (7, 5, 3, 2), (512, 8, 24, 1), (300, 100, 12, 3), (64, 4, 16, 0)]
+    for strides in layouts:
+        here = _addresses(shape, strides)
+        assert _shared(shape, strides, 0) == (len(set(here)) < len(here))
+        for apart in range(-60, 61):
+            if apart:
+                there = {a + apart for a in here}
+                assert _shared(shape, strides, apart) == (not there.isdisjoint(here)), (strides, apart)
+
+
+def test_overlapping_outputs_are_refused(on_cpu):
+    from lcv_bsa import cached_attention
+
+    c, q = _cache(), torch.zeros(2, 4, 3, 64, dtype=torch.bfloat16)
+    held = torch.zeros(4096, dtype=torch.bfloat16)
+    for strides in ((768, 192, 32, 1), (768, 128, 64, 1), (64, 192, 64, 1), (192, 192, 64, 1), (768, 192, 64, 0)):
+        with pytest.raises(ValueError, match="share"):
+            cached_attention(q, c, 5, out=held.as_strided(q.shape, strides))
+    for strides in ((768, 192, 64, 1), (768, 64, 256, 1), (200, 400, 66, 1), (1, 400, 2, 6)):
+        with pytest.raises(AssertionError, match="reached"):
+            cached_attention(q, c, 5, out=held.as_strided(q.shape, strides))
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="validation-only calls use fake pointers; CPU container only")
+def test_c_attention_in_place_has_the_same_strides():
+    from lcv_bsa import _lib
+
+    lib, fake = _lib.load(), 1 << 20
+    c = _lib.Cache8(k8=fake, v8=fake, k_scale=fake, v_scale=fake, B=1, H=2, capacity=128, D=64)
+    a, b = _lib.Strides(8192, 4096, 64), _lib.Strides(8192, 64, 128)
+    assert lib.lcv_bsa_cached_attn(fake, 1, 2, 4, a, c, fake, None, 0, 0.1, 64, fake, b, None, None, 0, None) == _lib.ERR_LAYOUT
+    assert b"in place" in lib.lcv_bsa_last_error()

@@ -1,5 +1,6 @@
 """The 8-bit cache beside what watches or changes a layer: norms of other kinds, forward-mode
-derivatives; refusals before any work; appending near the capacity."""
+derivatives; refusals before any work; outputs
+that share memory with the queries; appending near the capacity."""
 
 from __future__ import annotations
 
@@ -8,7 +9,7 @@ import torch
 from torch.autograd import forward_ad
 
 from conftest import NORM_CHANGES, changed_norms
-from test_gpu_kv_cache import BF16, F32, _gen, _ints, _stored
+from test_gpu_kv_cache import BF16, F32, _cache, _gen, _ints, _stored
 from test_gpu_kv_cache_layer import _layer
 
 pytestmark = pytest.mark.gpu
@@ -131,3 +132,31 @@ def test_refused_before_any_work(device, bsa, calls):
     with torch.no_grad():
         m(x, GRID, return_kv=True)
     assert any(seen)
+
+
+@pytest.mark.parametrize("S", [1, 4, 40, 130])
+def test_out_beside_q(device, S):
+    """out over q's memory, some rows on; out between q's rows."""
+    from lcv_bsa import cached_attention
+
+    gen = _gen(device, S)
+    B, H, D = 2, 4, 64
+    c = _cache(gen, device, B, H, 1024, D)
+    n = _ints(device, [1000, 70])
+    q = torch.randn(B, H, S, D, generator=gen, device=device).to(BF16)
+    want = cached_attention(q, c, n)
+    size = q.numel()
+    for shift in (8, 64, 3 * 64, 64 * S, -64):
+        held = torch.zeros(size + 2 * abs(shift), dtype=BF16, device=device)
+        a, b = (shift, 2 * shift) if shift > 0 else (-shift, 0)
+        src, to = held[a:a + size].view(B, H, S, D), held[b:b + size].view(B, H, S, D)
+        src.copy_(q)
+        assert cached_attention(src, c, n, out=to) is to and torch.equal(to, want)
+    held = torch.zeros(size, dtype=BF16, device=device)
+    src, to = held.view(B, H, S, D).copy_(q), held.view(B, S, H, D).transpose(1, 2)
+    assert torch.equal(cached_attention(src, c, n, out=to), want)
+    packed = torch.zeros(B, S, 3, H, D, dtype=BF16, device=device)
+    src, to = packed[:, :, 0].transpose(1, 2), packed[:, :, 1].transpose(1, 2)
+    src.copy_(q)
+    assert torch.equal(cached_attention(src, c, n, out=to), want)
+    assert torch.equal(src, q) and not packed[:, :, 2].any()
