@@ -17,6 +17,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 // lse in units of log2; where it is -inf every score is, and any finite number will do.
 __device__ __forceinline__ float offset_of(float lse) { return lse == -__builtin_inff() ? 0.0f : lse * kLog2e; }
 
+// What turns a block's products into scores: never zero, so that -inf stays -inf, as in the
+// attention.
+__device__ __forceinline__ float key_scale(const CacheAttn& a, int64_t block) {
+  const float c = a.scale_log2 * a.c.k_scale[block];
+  return c > 0x1p-126f ? c : 0x1p-126f;
+}
+
 template <typename T, int D>
 __device__ __forceinline__ void load_keys(const CacheAttn& a, int64_t block, int lane, typename Mfma<T>::vec8 (&kf)[4][D / 32]) {
   const uint8_t* kb = a.c.k8 + block * (64 * D) + lane % 16 * D + lane / 16 * (D / 4);
@@ -49,7 +56,7 @@ __global__ __launch_bounds__(256) void few_weights_kernel(CacheAttn a, const flo
   if (64 * j < n.len) {
     vec8 kf[4][D / 32];
     load_keys<T, D>(a, block, lane, kf);
-    const float c = a.scale_log2 * a.c.k_scale[block];
+    const float c = key_scale(a, block);
     for (int r0 = 0; r0 < rows; r0 += 16) {
       const int r = r0 + gi < rows ? r0 + gi : rows - 1;
       const T* q = reinterpret_cast<const T*>(a.q.ptr) + (int64_t)b * a.q.sb +
@@ -132,7 +139,7 @@ void many_weights_kernel(CacheAttn a, const float* w_in, float* w_out, float* pa
     float c = 0.0f;
     if (mine) {
       load_keys<T, D>(a, block, lane, kf);
-      c = a.scale_log2 * a.c.k_scale[block];
+      c = key_scale(a, block);
     } else {
 #pragma unroll
       for (int t = 0; t < 4; ++t)

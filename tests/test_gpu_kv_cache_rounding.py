@@ -108,6 +108,24 @@ def test_scores_far_below_a_first_block_of_minus_infinity(device, S):
     assert float((lse - (math.log(64) - 512)).abs().max()) <= 2.0 ** -13  # fp32 near 2^9: 2^-15 a rounding
 
 
+@pytest.mark.parametrize("S", [1, 100])
+@pytest.mark.parametrize("scale", [0.0, 1e-38])
+def test_weights_of_minus_infinity_under_a_small_scale(device, S, scale):
+    """Products that overflow are scores of -inf whatever the softmax scale, for the weights
+    as for the attention."""
+    from lcv_bsa import KVCache8, attention_weights, cache_append, cached_attention
+
+    k = torch.zeros(1, 1, 64, 64, device=device)
+    k[:, :, :40, 0] = -1.0  # stored as -256
+    c = cache_append(KVCache8.empty(1, 1, 64, 64, device), k, torch.ones_like(k), 0)
+    q = torch.zeros(1, 1, S, 64, dtype=BF16, device=device)
+    q[..., 0] = 2.0 ** 120
+    out, lse = cached_attention(q, c, 64, sm_scale=scale, return_lse=True)
+    assert bool((out == 1).all())
+    w = attention_weights(q, c, 64, lse, sm_scale=scale)[0, 0]
+    assert not w[:40].any() and float((w[40:] - S / 24).abs().max()) <= S / 24 * 2.0 ** -18
+
+
 @pytest.mark.parametrize("scale", [128 ** -0.5, 1.0])
 def test_sparse_queries_beside_an_unanswered_value(device, scale):
     """Walks of 32 blocks in bf16, D = 128: rows of one large value in a channel where keys
