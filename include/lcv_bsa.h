@@ -532,8 +532,8 @@ int lcv_bsa_cached_attn(const void* q, int dtype, int64_t Hq, int64_t S,
  * What each cached token got from these queries: out[b,h,j] = weights[b,h,j] +
  * the sum over the queries of key head h that see token j of exp(sm_scale q.k_j -
  * lse), with lse from lcv_bsa_cached_attn.  weights (null: zeros) and out are
- * [B,H,capacity] fp32, one buffer or two apart.  The sums' order is fixed.  The workspace
- * holds the sums of parts of the rows.
+ * [B,H,capacity] fp32, one buffer or two apart; lse lies apart from out.  The sums'
+ * order is fixed.  The workspace holds the sums of parts of the rows.
  */
 size_t lcv_bsa_attention_weights_workspace_bytes(int64_t Hq, int64_t S,
                                                  lcv_bsa_cache8 c,

@@ -1186,6 +1186,9 @@ int lcv_bsa_attention_weights(const void* q, int dtype, int64_t Hq, int64_t S, l
   const size_t need = lcv::cache_weights_workspace(a, (int)c.D);
   if (workspace_bytes < need || (need && (!workspace || (uintptr_t)workspace % 16)))
     return fail(LCV_BSA_ERR_INVALID_ARG, "workspace of %zu bytes, 16-byte aligned, needed (got %zu)", need, workspace_bytes);
+  const uintptr_t read = (uintptr_t)lse, read_bytes = (uintptr_t)c.B * (uintptr_t)Hq * (uintptr_t)S * sizeof(float);
+  if (read < to + bytes && to < read + read_bytes)
+    return fail(LCV_BSA_ERR_INVALID_ARG, "lse and out overlap");
   a.workspace = workspace;
   return launch_status(lcv::launch_cache_weights(a, dtype, (int)c.D, weights, out, (hipStream_t)stream),
                        "lcv_bsa_attention_weights");

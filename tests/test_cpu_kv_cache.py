@@ -348,3 +348,15 @@ def test_c_attention_in_place_has_the_same_strides():
     a, b = _lib.Strides(8192, 4096, 64), _lib.Strides(8192, 64, 128)
     assert lib.lcv_bsa_cached_attn(fake, 1, 2, 4, a, c, fake, None, 0, 0.1, 64, fake, b, None, None, 0, None) == _lib.ERR_LAYOUT
     assert b"in place" in lib.lcv_bsa_last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="validation-only calls use fake pointers; CPU container only")
+def test_c_weights_refuse_an_out_on_lse():
+    from lcv_bsa import _lib
+
+    lib, fake = _lib.load(), 1 << 20
+    st = _lib.Strides(8192, 4096, 64)
+    c = _lib.Cache8(k8=fake, v8=fake, k_scale=fake, v_scale=fake, B=1, H=2, capacity=128, D=64)
+    for apart in (0, 28, -1020):  # lse has 32 bytes, out 1024
+        assert lib.lcv_bsa_attention_weights(fake, 1, 2, 4, st, c, fake, None, 0, 0.1, 64, fake, None, fake + apart, None, 0, None) == _lib.ERR_INVALID_ARG
+        assert b"lse and out overlap" in lib.lcv_bsa_last_error()
