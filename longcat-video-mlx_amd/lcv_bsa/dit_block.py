@@ -142,7 +142,8 @@ class Attention(nn.Module, BSAAttention):
 
     ``kv_cache_8bit = True`` keeps the cache that ``return_kv`` asks for in 8 bits: a
     pair of a ``KVCache8`` (keys after RoPE; half the memory of the reference's, without
-    a gradient) and the number of its tokens; ``forward_with_kv_cache`` takes either kind."""
+    a gradient) and the number of its tokens; ``forward_with_kv_cache`` takes either kind,
+    for BSA too, which reads the cached keys and values widened to 16 bits."""
 
     def __init__(self, dim: int, num_heads: int, **kw):
         nn.Module.__init__(self)
@@ -263,7 +264,8 @@ class Attention(nn.Module, BSAAttention):
                        cached: int) -> torch.Tensor:
         """The continuation from an 8-bit cache of ``ncl`` frames: the new tokens are
         turned to their frames' positions and appended to a copy of it, and their
-        queries attend to all of it (densely, as the reference's do)."""
+        queries attend to all of it (densely, as the reference's do).  Where BSA runs
+        between cached and new frames, the cached ones are widened to x's dtype for it."""
         B, N, C = x.shape
         H, D = self.num_heads, self.head_dim
         T, Hl, Wl = (int(s) for s in shape)
@@ -271,19 +273,36 @@ class Attention(nn.Module, BSAAttention):
         if ncl <= 0 or N != T * Hl * Wl or b not in (1, B) or (h, d) != (H, D) or not cached == ncl * Hl * Wl <= n:
             raise ValueError(f"an 8-bit cache {cache.shape} of {cached} tokens does not hold {ncl} frames of {Hl} x {Wl} "
                              f"before {N} new tokens of {B} items, {H} heads of {D}")
-        q, k, v = (t.transpose(1, 2) for t in self.qkv(x).view(B, N, 3, H, D).unbind(2))
+        qkv = self.qkv(x).view(B, N, 3, H, D)
+        no_derivative("the continuation from an 8-bit cache", qkv, *self.q_norm.parameters(), *self.k_norm.parameters())
+        q, k, v = (t.transpose(1, 2) for t in qkv.unbind(2))
         if self._cache_fusible(q, k):
             q, k = (head_rms_norm(t, m.weight, m.eps) for t, m in ((q, self.q_norm), (k, self.k_norm)))
         else:
             q, k = self.q_norm(q), self.k_norm(k)
         positions = grid_positions((T, Hl, Wl), (ncl, 0, 0), x.device)
         q, k = (rope_nd(t, positions, rope_dims(D)) for t in (q, k))
-        cache = cache_append(cache.extended(max(n, cached + N), B), k, v, cached)
         o = torch.empty((B, N, H, D), dtype=x.dtype, device=x.device)
-        cached_attention(q, cache, cached + N, sm_scale=self.scale, out=o.transpose(1, 2))
-        self.last_indices, self.last_paths = {}, {"noise": "dense"}
-        self.last_path = "dense"
+        self.last_indices, self.last_paths = {}, {}
+        if self._continued_geometry(shape, ncl) is not None:
+            held = (t[:, :, :cached].expand(B, -1, -1, -1) for t in cache.dequantize(x.dtype))
+            k, v = (torch.cat([c, t], 2) for c, t in zip(held, (k, v)))
+            self._attend("noise", q, k, v, (T, Hl, Wl), kv_shape=(T + ncl, Hl, Wl), out=o.transpose(1, 2))
+        else:
+            cache = cache_append(cache.extended(max(n, cached + N), B), k, v, cached)
+            cached_attention(q, cache, cached + N, sm_scale=self.scale, out=o.transpose(1, 2))
+            self.last_path = self.last_paths["noise"] = "dense"
         return self.proj(o.view(B, N, C))
+
+    def _continued_geometry(self, shape: Sequence[int], ncl: int):
+        """What BSA goes by between the queries of ``shape`` and the keys of ``ncl`` cached
+        frames and theirs: (shape, voxel) of either; None where it does not run there."""
+        if not (self.enable_bsa and self.bsa_cond_noise and ncl > 0):
+            return None
+        validate_backend(self.bsa_backend)
+        T, Hl, Wl = (int(s) for s in shape)
+        gq, gk = (bsa_geometry((t, Hl, Wl), self.bsa_chunk_thw, self.bsa_shape_policy) for t in (T, T + ncl))
+        return None if gq is None or gk is None or gq[1] != gk[1] else (gq, gk)
 
     def _continue_fused(self, q, k, v, x, shape, ncl, kv_cache):
         """The continuation with BSA over cached + new keys, from one
@@ -291,16 +310,15 @@ class Attention(nn.Module, BSAAttention):
         k_cache, v_cache = kv_cache
         T, Hl, Wl = (int(s) for s in shape)
         B, H, N, D = q.shape
-        if not (self.enable_bsa and self.bsa_cond_noise and ncl > 0 and N == T * Hl * Wl
+        if not (N == T * Hl * Wl
                 and tuple(k_cache.shape) == tuple(v_cache.shape) == (k_cache.shape[0], H, ncl * Hl * Wl, D)
                 and k_cache.shape[0] in (1, B)
                 and self._cache_fusible(q, k_cache, v_cache)):
             return None
-        validate_backend(self.bsa_backend)
-        grid = (T + ncl, Hl, Wl)
-        gq, gk = (bsa_geometry(g, self.bsa_chunk_thw, self.bsa_shape_policy) for g in ((T, Hl, Wl), grid))
-        if gq is None or gk is None or gq[1] != gk[1]:
+        geometry = self._continued_geometry(shape, ncl)
+        if geometry is None:
             return None
+        (gq, gk), grid = geometry, (T + ncl, Hl, Wl)
         try:
             q, k, v, qb, kb = prepare_qkv(q, k, v, grid, gq[0], gk[0], gq[1], cache=(k_cache, v_cache),
                                           q_weight=self.q_norm.weight, k_weight=self.k_norm.weight,

@@ -1,6 +1,6 @@
 """The 8-bit cache beside what watches or changes a layer: norms of other kinds, forward-mode
-derivatives; refusals before any work; outputs
-that share memory with the queries; appending near the capacity."""
+derivatives, block-sparse continuations; refusals before any work; outputs that share memory
+with the queries; appending near the capacity."""
 
 from __future__ import annotations
 
@@ -160,3 +160,67 @@ def test_out_beside_q(device, S):
     src.copy_(q)
     assert torch.equal(cached_attention(src, c, n, out=to), want)
     assert torch.equal(src, q) and not packed[:, :, 2].any()
+
+
+@pytest.mark.parametrize("batch", [1, 2])
+@pytest.mark.parametrize("dtype", [torch.float16, BF16])
+def test_block_sparse_continuation(device, batch, dtype, monkeypatch):
+    """BSA between cached and new frames runs from an 8-bit cache as from a 16-bit one: over
+    the cached keys as they are stored and the new ones as they are."""
+    from lcv_bsa import dit_block
+
+    m = _layer(device, dtype, bsa=True)
+    more = torch.randn(batch, 192, 128 * 2, generator=_gen(device, 5), device=device).to(dtype)
+    x, shape = _input(device, dtype=dtype), (3,) + GRID[1:]
+    with torch.no_grad():
+        m.kv_cache_8bit = False
+        plain = m(x, GRID, return_kv=True)[1]
+        m.kv_cache_8bit = True
+        cache = m(x, GRID, return_kv=True)[1]
+        dense = m.forward_with_kv_cache(more, shape, 2, cache)
+        assert m.last_paths == {"noise": "dense"}
+        m.bsa_cond_noise, m.bsa_top_k, m.keep_indices = True, 5, True
+        near = lambda a, b: float((a.float() - b.float()).norm() / (b.float() - m.proj.bias.float()).norm()) < 2.0 ** -4  # noqa: E731
+        all_blocks = m.forward_with_kv_cache(more, shape, 2, cache)
+        assert m.last_paths == {"noise": "bsa"} and near(all_blocks, dense)
+        assert near(all_blocks, m.forward_with_kv_cache(more, shape, 2, plain))
+        m.bsa_top_k, seen, bsa = 2, [], dit_block.bsa_attention
+
+        def watched(q, k, v, *args, **kw):
+            seen.append((q, k, v, kw))
+            return bsa(q, k, v, *args, **kw)
+
+        monkeypatch.setattr(dit_block, "bsa_attention", watched)
+        out = m.forward_with_kv_cache(more, shape, 2, cache)
+    (q, k, v, kw), = seen
+    for got, held in zip((k, v), cache[0].dequantize(dtype)):
+        assert got.shape == (batch, 2, 320, 128) and torch.equal(got[:, :, :128], held.expand(batch, -1, -1, -1))
+    assert kw["kv_shape"] == (5, 8, 8) or kw["kv_shape"] == (1, 1, 320)
+    idx = m.last_indices["noise"]
+    assert idx.shape[-1] == 2
+    # Each block of 64 queries over the keys of its two blocks, in 64 bits on the CPU; P and
+    # the output are rounded to 16 bits, and so is the projection's input.
+    want = torch.zeros(batch, 192, 2, 128, dtype=torch.float64)
+    q, k, v, idx = (t.cpu() for t in (q.double(), k.double(), v.double(), idx.long()))
+    for b in range(batch):
+        for h in range(2):
+            for i in range(3):
+                at = (idx[b, h, i][:, None] * 64 + torch.arange(64)).flatten()
+                s = q[b, h, 64 * i:64 * i + 64] @ k[b, h, at].T.contiguous() * 128 ** -0.5
+                want[b, 64 * i:64 * i + 64, h] = torch.softmax(s, -1) @ v[b, h, at]
+    want = want.flatten(2) @ m.proj.weight.detach().cpu().double().T + m.proj.bias.detach().cpu().double()
+    assert float((out.cpu().double() - want).norm() / want.norm()) < 2.0 ** -6
+
+
+def test_continuation_with_gradients_is_refused(device, calls):
+    from lcv_bsa import dit_block
+
+    m, x = _layer(device, bsa=True), _input(device)
+    more = torch.randn(1, 192, 256, generator=_gen(device, 5), device=device).to(BF16)
+    with torch.no_grad():
+        cache = m(x, GRID, return_kv=True)[1]
+    seen = [calls(dit_block, name) for name in ("bsa_attention", "cached_attention", "rope_nd", "cache_append")]
+    for m.bsa_cond_noise in (False, True):
+        with pytest.raises(ValueError, match="backward"):
+            m.forward_with_kv_cache(more, (3, 8, 8), 2, cache)
+    assert not any(seen)
