@@ -302,7 +302,7 @@ void few_rows_kernel(CacheAttn a, Parts p) {
         t = Mfma<T>::mma(v0, pf[nt][0], t);
         t = Mfma<T>::mma(v1, pf[nt][1], t);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[nt][dt][i] = __builtin_fmaf(o[nt][dt][i], down[nt], t[i] * up[nt]);
+        for (int i = 0; i < 4; ++i) o[nt][dt][i] = __builtin_fmaf(t[i], up[nt], o[nt][dt][i] * down[nt]);
       }
       ask_v(jn, dt);
     }
