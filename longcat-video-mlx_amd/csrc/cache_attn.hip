@@ -507,7 +507,7 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 // and a row's values as the sum of two e4m3 numbers under the row's 2^e and 2^(e - 4): two
 // passes at twice bf16's rate, and 64 conversions less.  e4m3's 4 bits twice are bf16's 8,
 // so that values from 2^(e - 6) on (2^-14.8 of the row's largest) are exact; one below is
-// off by no more than 2^(e - 14), nor than itself.  What that adds up to in a score, if
+// off by no more than 2^(e - 14).  What that adds up to in a score, if
 // every key held its scale's largest number there, has to stay below kLost in u for all
 // rows of the workgroup (normed rows of 128 against normed keys: 2^-20 for each such value,
 // of which a row has 0.02), else it converts the keys: a row whose largest value is far
@@ -529,32 +529,30 @@ constexpr bool kIsBf16 = false;
 template <>
 constexpr bool kIsBf16<bf16> = true;
 
-// The largest key scale of blocks j0 .. j1 - 1.
-__device__ __forceinline__ float largest_scale(const float* ksc, int j0, int j1) {
-  float most = 0.0f;
-  for (int j = j0 + threadIdx.x % 64; j < j1; j += 64) most = fmaxf(most, ksc[j]);
-  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
-  return most;
-}
-
 // Of blocks j0 .. j1 - 1: the largest exponent of a value scale below `below`, and the
-// least one; without any, one below and one above the range.
+// least one; without any, one below and one above the range.  With KEYS, the largest key
+// scale too.
 struct Span {
   int top, least;
+  float key;
 };
-__device__ __forceinline__ Span span_of(const float* vsc, int j0, int j1, int below) {
-  Span s = {-kMaxScaleExp - 1, kMaxScaleExp + 1};
+template <bool KEYS>
+__device__ __forceinline__ Span span_of(const float* ksc, const float* vsc, int j0, int j1, int below) {
+  Span s = {-kMaxScaleExp - 1, kMaxScaleExp + 1, 0.0f};
   for (int j = j0 + threadIdx.x % 64; j < j1; j += 64) {
+    const float key = KEYS ? ksc[j] : 0.0f;
     const int e = exponent_of(vsc[j]);
     s.top = e < below && e > s.top ? e : s.top;
     s.least = e < s.least ? e : s.least;
+    s.key = fmaxf(s.key, key);
   }
   for (int o = 1; o < 64; o <<= 1) {
     const int t = __shfl_xor(s.top, o), l = __shfl_xor(s.least, o);
     s.top = t > s.top ? t : s.top;
     s.least = l < s.least ? l : s.least;
+    if constexpr (KEYS) s.key = fmaxf(s.key, __shfl_xor(s.key, o));
   }
-  return {uniform_i32(s.top), uniform_i32(s.least)};
+  return {uniform_i32(s.top), uniform_i32(s.least), s.key};
 }
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 constexpr float kLost = 0x1p-14f;
@@ -605,7 +603,8 @@ void many_rows_kernel(CacheAttn a, Parts p) {
   const int j0 = split * p.per;
   const int j1 = j0 + p.per < nblk ? j0 + p.per : nblk;
   if (split > 0 && j0 >= nblk) return;  // the first part of a tile always answers
-  const Span span = span_of(a.c.v_scale + (int64_t)bh * a.c.nb, j0, j1, kMaxScaleExp + 1);
+  const Span span = span_of<kBytes>(a.c.k_scale + (int64_t)bh * a.c.nb, a.c.v_scale + (int64_t)bh * a.c.nb, j0, j1,
+                                    kMaxScaleExp + 1);
   const Reach mine = reach(a, n, kRows * tile + 32 * wave, kRows * tile + 32 * wave + 32);
   const int own = uniform_i32(mine.most), least = uniform_i32(mine.least);
 
@@ -916,7 +915,7 @@ void many_rows_kernel(CacheAttn a, Parts p) {
           const int e = value_exponent(j);
           if (mine(j, e)) block(j, slot, e, Flag<true>{}, Flag<true>{});
         }
-        band = span_of(vsc, j0, j1, band - kSpread<T>).top;
+        band = span_of<false>(ksc, vsc, j0, j1, band - kSpread<T>).top;
         if (band < span.least) break;
         __syncthreads();  // the ring is free
       }
@@ -999,19 +998,19 @@ void many_rows_kernel(CacheAttn a, Parts p) {
     }
   };
   if constexpr (kBytes) {
-    const float answer = 448.0f * a.scale_log2 * largest_scale(a.c.k_scale + (int64_t)bh * a.c.nb, j0, j1);
     bool fine = true;
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
-      const float unit = pow2i(byte_exponent<D>(qf[qt]));
-      float lost = 0.0f;
+      const int e = byte_exponent<D>(qf[qt]);
+      const float bound = 0x1p-6f * pow2i(e);
+      float small = 0.0f;  // values that may be off
 #pragma unroll
       for (int x = 0; x < D / 4; ++x) {
         const float y = __builtin_fabsf(to_f32(qf[qt][x / 8][x % 8]));
-        if (y < 0x1p-6f * unit) lost += fminf(y, 0x1p-14f * unit);
-        if (y == __builtin_inff()) lost = y;
+        small += y != 0.0f && y < bound ? 1.0f : 0.0f;
       }
-      fine = fine && sum_quarters(lost) * answer <= kLost;  // false for a NaN
+      const float lost = sum_quarters(small) * (0x1p-8f * bound) * (448.0f * span.key) * a.scale_log2;
+      fine = fine && e < 120 && lost <= kLost;  // false for an infinite value, and for a NaN
     }
     if (!__syncthreads_or(!fine)) {
       rest(Flag<true>{});
