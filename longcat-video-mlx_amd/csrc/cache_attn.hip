@@ -488,14 +488,16 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 //   P' = exp2(u + ev - m),  O = sum P' v8,  l = sum 2^(least - ev) P',  least the least ev,
 // so that O holds the true sum over 2^m and l the softmax's denominator over 2^(m - least).
 // A row's offset m comes from its first half block, and later halves need no maximum: in
-// bf16 that of u + ev, in fp16 that of u plus least, so that P' is no less than a token's
-// weight against the half's heaviest.  Where a half's sum passes a bound (fp16's largest
-// number; 2^40 in bf16), or is NaN, or the half's scores are all -inf, or the value scales
-// are more than 2^kSpread apart, the workgroup walks with care: band by band of scales so
-// close, each walked once for the rows' maxima of u + ev and once for its products, and O
-// and l brought from band to band.  The next band's offset lies no more than kFar below the
-// largest so far, which leaves O room in fp32.  (Rescaling O inside the walk costs it 60
-// registers: 4310 us, below 3600.)
+// bf16 that of u + ev, in fp16 that of u plus least (or plus the largest ev less kLift, if
+// that is more), so that P' is no less than a token's weight against the half's heaviest (or
+// 2^-3 of it).  Where a half's sum passes a bound (fp16's largest number; 2^40 in bf16), or
+// is NaN, or the half's scores are all -inf, or the value scales are more than 2^kSpread
+// apart, the workgroup walks with care: band by band of scales so close, each walked once
+// for the rows' maxima of u + ev and once for its products, and O and l brought from band
+// to band.  The next band's offset lies no more than kFar below the largest so far, which
+// leaves O room in fp32.  (Rescaling O inside the walk costs it 60 registers: 4310 us, below
+// 3600.)  12,480 fp16 queries of 32 heads over 18,720 tokens take 3670 us, beside one value
+// that is 2^16 times the others 6990, with scores that pass the bound 9390.
 //
 // Bound by instructions: a block costs a wave 64 MFMAs (1024 cycles), 32 exponentials with
 // their sums and 128 conversions of bytes, about 2350 cycles with the MFMAs beside them.
@@ -507,11 +509,11 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 // and a row's values as the sum of two e4m3 numbers under the row's 2^e and 2^(e - 4): two
 // passes at twice bf16's rate, and 64 conversions less.  e4m3's 4 bits twice are bf16's 8,
 // so that values from 2^(e - 6) on (2^-14.8 of the row's largest) are exact; one below is
-// off by no more than 2^(e - 14).  What that adds up to in a score, if
-// every key held its scale's largest number there, has to stay below kLost in u for all
-// rows of the workgroup (normed rows of 128 against normed keys: 2^-20 for each such value,
-// of which a row has 0.02), else it converts the keys: a row whose largest value is far
-// above the rest, which its keys may not answer, or an infinite one.
+// off by no more than 2^(e - 14).  What that adds up to in a score, if every key held its
+// scale's largest number there, has to stay below kLost in u for all rows of the workgroup
+// (normed rows of 128 against normed keys: 2^-20 for each such value, of which a row has
+// 0.02), else it converts the keys: a row whose largest value is far above the rest, which
+// its keys may not answer, or an infinite one.
 // 12,480 queries of 32 heads over 18,720 tokens then take 3376 us, 1134 TFLOP/s, against
 // 3637 (a product of 8192^3 makes 1214); 2048 over 2048 of 32 heads 75 against 78.
 template <typename T>
@@ -521,7 +523,8 @@ constexpr float kMaxSum<f16> = 65504.0f;
 template <typename T>
 constexpr int kSpread = 32;
 template <>
-constexpr int kSpread<f16> = 8;
+constexpr int kSpread<f16> = 12;
+constexpr int kLift = 9;
 constexpr float kFar = 80.0f;
 
 template <typename T>
@@ -803,8 +806,9 @@ void many_rows_kernel(CacheAttn a, Parts p) {
     auto value_exponent = [&](int j) {
       return exponent_of(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs64), j & 63)));
     };
+    const float lifted = (float)(span.top - kLift > span.least ? span.top - kLift : span.least);
     bool dirty = false;
-    // kCareful: the offsets are known; every block counts as one that rows see in part.
+    // careful: the offsets are known.
     auto block = [&](int j, int slot, int e, auto kind, auto how) {
       constexpr bool part = decltype(kind)::value;  // some row of the wave sees the block in part
       constexpr bool careful = decltype(how)::value;
@@ -816,7 +820,7 @@ void many_rows_kernel(CacheAttn a, Parts p) {
         if constexpr (part) mask(j, h);
         if constexpr (!careful) {
           if (h == 0 && j == j0) {
-            raise(h, c, kIsBf16<T> ? ev : (float)span.least);
+            raise(h, c, kIsBf16<T> ? ev : lifted);
             if (__ballot((m[0] == kNegInf && vis[0] > 64 * j0) || (m[1] == kNegInf && vis[1] > 64 * j0))) dirty = true;
           }
         }
@@ -831,7 +835,7 @@ void many_rows_kernel(CacheAttn a, Parts p) {
       }
     };
     // Blocks before `whole` are seen whole by every row of the wave that sees any token.
-    int whole = own == 0 ? 0 : least / 64 < j1 ? least / 64 : j1;
+    const int whole = own == 0 ? 0 : least / 64 < j1 ? least / 64 : j1;
     int j, slot;
     auto begin = [&] {
       j = j0, slot = 0;
@@ -874,7 +878,6 @@ void many_rows_kernel(CacheAttn a, Parts p) {
       if (careful) clear();
     }
     if (careful) {
-      whole = j0;
       float reached[2] = {kNegInf, kNegInf};  // the largest u + ev so far
       for (int band = span.top;;) {           // value scales of kSpread exponents up to `band`
         auto mine = [&](int j, int e) { return 64 * j < own && e <= band && e >= band - kSpread<T>; };
@@ -888,7 +891,7 @@ void many_rows_kernel(CacheAttn a, Parts p) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             qk(ring + slot * kSlot, h);
-            mask(j, h);
+            if (j >= whole) mask(j, h);
             raise(h, key_scale(j), (float)e);
           }
         }
@@ -910,6 +913,11 @@ void many_rows_kernel(CacheAttn a, Parts p) {
             for (int i = 0; i < 4; ++i) o[dt][qt][i] *= f;
         }
         begin();
+        for (; j < whole; ++j, slot = slot == 2 ? 0 : slot + 1) {
+          next();
+          const int e = value_exponent(j);
+          if (mine(j, e)) block(j, slot, e, Flag<false>{}, Flag<true>{});
+        }
         for (; j < j1; ++j, slot = slot == 2 ? 0 : slot + 1) {
           next();
           const int e = value_exponent(j);

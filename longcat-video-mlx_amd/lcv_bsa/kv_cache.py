@@ -289,7 +289,7 @@ def cached_attention(q: torch.Tensor, cache: KVCache8, lengths: Ints, *, q_lens:
     short histories in a long cache.
 
     Sums are fp32.  Before they meet the values, probabilities are rounded to q's type
-    once: by half a step of it, in fp16 by up to 2^-25 of the row's largest, however far
+    once: by half a step of it, in fp16 by up to 2^-22 of the row's largest, however far
     apart the blocks' scales are.  A token whose weight is below 2^-40 of the heaviest's
     may be left out of the row's sum.
 
