@@ -116,7 +116,10 @@ constexpr int kRoom<f16> = 12;
 // of 128 (345 MB), takes 68 us with the join's 5, 5.1 TB/s (a copy of 1 GiB: 5.0); one over
 // 501 tokens 5.3 us, its loads' latency.  The next block's operands need the registers of
 // three waves a SIMD for 16 rows (74 us; two 79, four 111) and of two for 32 (24 rows of 8
-// heads over 9000 tokens 17 us; three 27).
+// heads over 9000 tokens 17 us; three 27).  In the joining of the waves' parts all 16 rows
+// of part_o lie in the same banks (0.8 of the LDS's active cycles): 1.4 % of the waves'
+// cycles go by waiting for it over long histories, 12 % where a wave walks two blocks (6
+// tokens of 4 requests, 17 us).
 template <typename T, int D, int NT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 1 ? 3 : 2, NT == 1 ? 3 : 2)))
 void few_rows_kernel(CacheAttn a, Parts p) {
@@ -481,8 +484,9 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 // of values (D = 128) go straight from memory into a ring of three LDS slots, two
 // blocks ahead, one barrier a block; every wave turns the bytes into T as it reads
 // them.  Operands as in few_rows_kernel.  LDS rows are 64 or 128 bytes in chunks of 16,
-// chunk c of row r at c ^ swz(r), so that the 16 rows that a lane group reads at once
-// lie in different banks.
+// chunk c of row r at c ^ swz(r), which spreads the 16 rows that a lane group reads over
+// the banks.  (Conflicts still take half of the LDS's active cycles, which access causes
+// them is not known; the waves wait for it in 1 % of theirs.)
 //
 // Here the value scale 2^ev is added to the exponent,
 //   P' = exp2(u + ev - m),  O = sum P' v8,  l = sum 2^(least - ev) P',  least the least ev,
@@ -514,8 +518,9 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 // (normed rows of 128 against normed keys: 2^-20 for each such value, of which a row has
 // 0.02), else it converts the keys: a row whose largest value is far above the rest, which
 // its keys may not answer, or an infinite one.
-// 12,480 queries of 32 heads over 18,720 tokens then take 3376 us, 1134 TFLOP/s, against
-// 3637 (a product of 8192^3 makes 1214); 2048 over 2048 of 32 heads 75 against 78.
+// 12,480 queries of 32 heads over 18,720 tokens then take 3380 us, 1132 TFLOP/s, against
+// 3710 (a product of 8192^3 makes 1214; 3290 to 3500 on other cards of the kind); 2048 over
+// 2048 of 32 heads 80 against 83.
 template <typename T>
 constexpr float kMaxSum = 0x1p40f;
 template <>

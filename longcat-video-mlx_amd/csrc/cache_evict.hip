@@ -15,8 +15,9 @@
 // whose bytes lie token by token, a wave takes one of the D rows at a time, its lanes the
 // 64 tokens: kept tokens are in order, so the lanes' bytes are in few lines.
 //
-// 9360 of 18,720 tokens of 32 heads of 128: ranking 17 us (32 workgroups, bound by the
-// passes' latency), gathering 40 us: 192 MB, as of the values every line is read, 4.8 TB/s.
+// 9360 of 18,720 tokens of 32 heads of 128: ranking 18 us (32 workgroups, bound by the
+// passes' latency), gathering 49 us: 192 MB, as of the values every line is read, 3.9 TB/s
+// (40 us from the last-level cache).
 #include "cache_common.h"
 
 namespace lcv {

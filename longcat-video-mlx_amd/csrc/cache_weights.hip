@@ -40,7 +40,8 @@ __device__ __forceinline__ void load_keys(const CacheAttn& a, int64_t block, int
 // Few rows (up to kFewRows a key head, row r = query r / group of head r % group): a
 // pass over the keys, one block a wave; the rows come from L2, 16 at a time.  Bound by the
 // keys' bytes: one token of 4 requests over 45,480 tokens of 8 heads of 128 (49 MB) takes
-// 13.8 us, 3.6 TB/s (four waves a SIMD; with the registers of five 19.5).
+// 14 to 15 us, 3.4 TB/s (four waves a SIMD; with the registers of five 5 us more): a wave
+// waits for its one block with nothing beside it.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void few_weights_kernel(CacheAttn a, const float* w_in, float* w_out) {
   typedef typename Mfma<T>::vec8 vec8;
@@ -98,15 +99,17 @@ __global__ __launch_bounds__(256) void few_weights_kernel(CacheAttn a, const flo
 // ring of three LDS slots, two tiles ahead, one barrier a tile; LDS rows in chunks of 16
 // bytes, chunk c of row r at c ^ kswz(r) (attn_common.h).  The exponentials (24 cycles an
 // element against 8 of its MFMAs) are the bound: 3120 rows of 32 heads of 128 over 9360
-// tokens take 256 us, 935 TFLOP/s.  Four waves a SIMD hide them (three: 260; D = 64, 3000
-// rows of 16 heads over 9000 tokens: 103 and 110).
+// tokens take 250 us, 957 TFLOP/s, the adding of parts with them; for D = 64 they are twice
+// as many for the same products (3000 rows of 16 heads over 9000 tokens 106 us, 520
+// TFLOP/s).  Four waves a SIMD hide them (260 and 110 with three, against 256 and 103).
+// Bank conflicts take 0.44 of the LDS's active cycles, waiting for it 0.6 % of the waves'.
 template <typename T, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4)))
 void many_weights_kernel(CacheAttn a, const float* w_in, float* w_out, float* parts, int splits) {
   typedef typename Mfma<T>::vec8 vec8;
   typedef MfmaCfg<T, D> C;
   constexpr int kRows = 32, kRowBytes = 2 * D;
-  constexpr int kTile = kRows * kRowBytes, kSlot = kTile + 256;  // the rows, then their lse
+  constexpr int kTile = kRows * kRowBytes;
   constexpr int kLoads = kTile / 4096;                          // 1 KB loads of a wave
   __shared__ __attribute__((aligned(1024))) uint8_t ring[3 * kTile];
   __shared__ __attribute__((aligned(1024))) float ring_lse[3][64];
