@@ -1152,7 +1152,7 @@ int lcv_bsa_cached_attn(const void* q, int dtype, int64_t Hq, int64_t S, lcv_bsa
   if (st) return st;
   if (!out) return fail(LCV_BSA_ERR_INVALID_ARG, "null pointer");
   if ((st = check_rows("out", out, os, c.D))) return st;
-  if (q == out && (qs.b != os.b || qs.h != os.h || qs.s != os.s))
+  if (q == out && ((c.B > 1 && qs.b != os.b) || (Hq > 1 && qs.h != os.h) || (S > 1 && qs.s != os.s)))
     return fail(LCV_BSA_ERR_LAYOUT, "in place, q and out must have the same strides");
   a.out = tensor4(out, os);
   a.lse = lse;

@@ -346,6 +346,11 @@ def test_c_attention_in_place_has_the_same_strides():
     lib, fake = _lib.load(), 1 << 20
     c = _lib.Cache8(k8=fake, v8=fake, k_scale=fake, v_scale=fake, B=1, H=2, capacity=128, D=64)
     a, b = _lib.Strides(8192, 4096, 64), _lib.Strides(8192, 64, 128)
+    # Strides of a dimension of size one say nothing: such a call goes on to its workspace.
+    long = _lib.Cache8(k8=fake, v8=fake, k_scale=fake, v_scale=fake, B=1, H=2, capacity=4096, D=64)
+    for S, same in ((4, _lib.Strides(64, 4096, 64)), (1, _lib.Strides(8192, 4096, 128))):
+        assert lib.lcv_bsa_cached_attn(fake, 1, 2, S, a, long, fake, None, 0, 0.1, 4096, fake, same, None, None, 0, None) == _lib.ERR_INVALID_ARG
+        assert b"workspace" in lib.lcv_bsa_last_error()
     assert lib.lcv_bsa_cached_attn(fake, 1, 2, 4, a, c, fake, None, 0, 0.1, 64, fake, b, None, None, 0, None) == _lib.ERR_LAYOUT
     assert b"in place" in lib.lcv_bsa_last_error()
 
