@@ -94,6 +94,24 @@ def test_value_scales_far_apart_in_whole_walks(device, kind, D):
                least=2.0 ** (-22 if kind == "near" else -25))
 
 
+@pytest.mark.parametrize("kind", ["far", "far, rising", "near", "outlier, 2e-3"])
+@pytest.mark.parametrize("size", [1.0, 12.0])
+def test_value_scales_far_apart_in_long_walks(device, kind, size):
+    """Walks of 33 blocks of D = 128, for bf16 the form that keeps the keys' bytes; scores
+    that pass the room of the first offset in fp16; queries that see the last block in part."""
+    from lcv_bsa import KVCache8, cache_append, cached_attention
+
+    gen = _gen(device, 8)
+    H, S, D, n = 512, 130, 128, 2100
+    v, dtype = _values(kind, gen, device, H, n, D)
+    k = torch.randn(1, H, n, D, generator=gen, device=device)
+    c = cache_append(KVCache8.empty(1, H, n, D, device), k, v, 0)
+    q = size * _rows(gen, device, 1, H, S, D, dtype)
+    out, lse = cached_attention(q, c, n - 3, return_lse=True)
+    for h in (0, H - 1):
+        _judge(q[:, h:h + 1], _head(c, h), [n - 3], out[:, h:h + 1], lse[:, h:h + 1], least=2.0 ** (-22 if kind == "near" else -25))
+
+
 @pytest.mark.parametrize("S", [1, 100])
 def test_scores_far_below_a_first_block_of_minus_infinity(device, S):
     """The first block's products overflow to -inf; what is left has the whole weight,
