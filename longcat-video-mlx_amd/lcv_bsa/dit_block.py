@@ -285,7 +285,10 @@ class Attention(nn.Module, BSAAttention):
         o = torch.empty((B, N, H, D), dtype=x.dtype, device=x.device)
         self.last_indices, self.last_paths = {}, {}
         if self._continued_geometry(shape, ncl) is not None:
-            held = (t[:, :, :cached].expand(B, -1, -1, -1) for t in cache.dequantize(x.dtype))
+            held = cache.dequantize(x.dtype)
+            if x.dtype == torch.float16:  # whose largest numbers may have been rounded up to 2^16
+                held = (t.clamp_(-65504.0, 65504.0) for t in held)
+            held = (t[:, :, :cached].expand(B, -1, -1, -1) for t in held)
             k, v = (torch.cat([c, t], 2) for c, t in zip(held, (k, v)))
             self._attend("noise", q, k, v, (T, Hl, Wl), kv_shape=(T + ncl, Hl, Wl), out=o.transpose(1, 2))
         else:

@@ -212,6 +212,26 @@ def test_block_sparse_continuation(device, batch, dtype, monkeypatch):
     assert float((out.cpu().double() - want).norm() / want.norm()) < 2.0 ** -6
 
 
+def test_block_sparse_continuation_of_the_largest_values(device):
+    """fp16's largest numbers round up to 2^16 in e4m3: widened, they are fp16's largest."""
+    from lcv_bsa import KVCache8, cache_append
+
+    m = _layer(device, torch.float16, bsa=True)
+    gen = _gen(device, 6)
+    more = torch.randn(1, 192, 256, generator=gen, device=device).to(torch.float16)
+    k, v = (torch.randn(1, 2, 128, 128, generator=gen, device=device) for _ in range(2))
+    v[:, :, 10, 3], v[:, 1, 70, 100], k[:, :, 30, 5] = 65504.0, -65000.0, 65504.0
+    cache = cache_append(KVCache8.empty(1, 2, 128, 128, device), k, v, 0)
+    with torch.no_grad():
+        m.proj.weight.mul_(2.0 ** -6)
+        m.bsa_cond_noise, m.bsa_top_k = True, 5
+        out = m.forward_with_kv_cache(more, (3, 8, 8), 2, (cache, 128))
+        assert m.last_paths == {"noise": "bsa"} and bool(torch.isfinite(out).all())
+        m.bsa_cond_noise = False
+        want = m.forward_with_kv_cache(more, (3, 8, 8), 2, (cache, 128)).float()
+    assert float((out.float() - want).norm() / want.norm()) < 2.0 ** -4
+
+
 def test_continuation_with_gradients_is_refused(device, calls):
     from lcv_bsa import dit_block
 
