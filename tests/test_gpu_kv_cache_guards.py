@@ -232,6 +232,36 @@ def test_block_sparse_continuation_of_the_largest_values(device):
     assert float((out.float() - want).norm() / want.norm()) < 2.0 ** -4
 
 
+def test_captured_block_sparse_continuation(device):
+    """Captured once, replayed with other latents and another clip's cache."""
+    from test_gpu_kv_cache_layer import _parts
+
+    m, shape = _layer(device, bsa=True), (3, 8, 8)
+    m.bsa_cond_noise, m.bsa_top_k = True, 3
+    frames = lambda seed, n: torch.randn(1, n, 256, generator=_gen(device, seed), device=device).to(BF16)  # noqa: E731
+    with torch.no_grad():
+        caches = [m(frames(s, 128), GRID, return_kv=True)[1] for s in (1, 2)]
+        held, x = m(frames(1, 128), GRID, return_kv=True)[1], frames(3, 192)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            m.forward_with_kv_cache(x, shape, 2, held)
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m.forward_with_kv_cache(x, shape, 2, held)
+        assert m.last_paths == {"noise": "bsa"}
+        for step in range(4):
+            x.copy_(frames(20 + step, 192))
+            for a, b in zip(_parts(held[0]), _parts(caches[step % 2][0])):
+                a.copy_(b)
+            graph.replay()
+            want = m.forward_with_kv_cache(x, shape, 2, caches[step % 2])
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+
+
 def test_continuation_with_gradients_is_refused(device, calls):
     from lcv_bsa import dit_block
 
