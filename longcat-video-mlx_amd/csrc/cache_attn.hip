@@ -611,8 +611,13 @@ void many_rows_kernel(CacheAttn a, Parts p) {
   const int j0 = split * p.per;
   const int j1 = j0 + p.per < nblk ? j0 + p.per : nblk;
   if (split > 0 && j0 >= nblk) return;  // the first part of a tile always answers
-  const Span span = span_of<kBytes>(a.c.k_scale + (int64_t)bh * a.c.nb, a.c.v_scale + (int64_t)bh * a.c.nb, j0, j1,
-                                    kMaxScaleExp + 1);
+  // One wave's reading decides for all, as barriers go by it.
+  __shared__ Span wave_span;
+  if (tid < 64) {
+    const Span s = span_of<kBytes>(a.c.k_scale + (int64_t)bh * a.c.nb, a.c.v_scale + (int64_t)bh * a.c.nb, j0, j1,
+                                   kMaxScaleExp + 1);
+    if (tid == 0) wave_span = s;
+  }
   const Reach mine = reach(a, n, kRows * tile + 32 * wave, kRows * tile + 32 * wave + 32);
   const int own = uniform_i32(mine.most), least = uniform_i32(mine.least);
 
@@ -628,6 +633,8 @@ void many_rows_kernel(CacheAttn a, Parts p) {
       qf[qt][ks] = __builtin_bit_cast(
           vec8, vis[qt] > 0 ? *reinterpret_cast<const u32x4*>(q + 8 * ks) : u32x4{0u, 0u, 0u, 0u});
   }
+  __syncthreads();
+  const Span span = {uniform_i32(wave_span.top), uniform_i32(wave_span.least), wave_span.key};
   __shared__ int wave_dirty[4];
   auto rest = [&](auto form) __attribute__((always_inline)) {
     constexpr bool bytes = decltype(form)::value;
@@ -928,9 +935,11 @@ void many_rows_kernel(CacheAttn a, Parts p) {
           const int e = value_exponent(j);
           if (mine(j, e)) block(j, slot, e, Flag<true>{}, Flag<true>{});
         }
-        band = span_of<false>(ksc, vsc, j0, j1, band - kSpread<T>).top;
-        if (band < span.least) break;
+        const int lower = span_of<false>(ksc, vsc, j0, j1, band - kSpread<T>).top;
+        if (tid == 0) wave_span.top = lower;
         __syncthreads();  // the ring is free
+        band = uniform_i32(wave_span.top);
+        if (band < span.least) break;
       }
     }
     if (nan_found) {  // wave-uniform, rare: rows that see a NaN among the values get one
