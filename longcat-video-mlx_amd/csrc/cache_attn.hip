@@ -519,7 +519,7 @@ __device__ __forceinline__ Turn by_length(const CacheAttn& a, int tiles, int r) 
 // 0.02), else it converts the keys: a row whose largest value is far above the rest, which
 // its keys may not answer, or an infinite one.
 // 12,480 queries of 32 heads over 18,720 tokens then take 3380 us, 1132 TFLOP/s, against
-// 3710 (a product of 8192^3 makes 1214; 3290 to 3500 on other cards of the kind); 2048 over
+// 3710 (a product of 8192^3 makes 1214; 3250 to 3500 from card to card); 2048 over
 // 2048 of 32 heads 80 against 83.
 template <typename T>
 constexpr float kMaxSum = 0x1p40f;

@@ -1,4 +1,4 @@
-"""What the attention over an 8-bit cache may lose to rounding, judged number by number:
+"""What the attention over an 8-bit cache may lose to rounding, number by number:
 value scales far apart, channels that only some blocks fill, queries beside large values
 that no key answers."""
 
@@ -21,7 +21,7 @@ def _head(c, h):
     return KVCache8(*(t[:, h:h + 1].clone(memory_format=torch.contiguous_format) for t in (c.k8, c.v8, c.k_scale, c.v_scale)))
 
 
-def _judge(q, c, lengths, out, lse, sm_scale=None, least=2.0 ** -25):
+def _check(q, c, lengths, out, lse, sm_scale=None, least=2.0 ** -25):
     """Each channel by what its own values carry: P is rounded to q's type once (half a step
     u of each; in fp16 no less than `least` of the row's largest, below which it is
     subnormal), the output once, and the scores' fp32 sums as R.attention has them."""
@@ -73,7 +73,7 @@ def test_value_scales_far_apart(device, kind, S, D):
     c = cache_append(KVCache8.empty(1, 1, n, D, device), k, v, 0)
     q = _rows(gen, device, 1, 1, S, D, dtype)
     out, lse = cached_attention(q, c, n - 5, return_lse=True)
-    _judge(q, c, [n - 5], out, lse, least=2.0 ** (-22 if kind == "near" else -25))
+    _check(q, c, [n - 5], out, lse, least=2.0 ** (-22 if kind == "near" else -25))
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -90,7 +90,7 @@ def test_value_scales_far_apart_in_whole_walks(device, kind, D):
     q = _rows(gen, device, 1, H, S, D, dtype)
     out, lse = cached_attention(q, c, n - 3, return_lse=True)
     for h in (0, H - 1):
-        _judge(q[:, h:h + 1], _head(c, h), [n - 3], out[:, h:h + 1], lse[:, h:h + 1],
+        _check(q[:, h:h + 1], _head(c, h), [n - 3], out[:, h:h + 1], lse[:, h:h + 1],
                least=2.0 ** (-22 if kind == "near" else -25))
 
 
@@ -109,7 +109,7 @@ def test_value_scales_far_apart_in_long_walks(device, kind, size):
     q = size * _rows(gen, device, 1, H, S, D, dtype)
     out, lse = cached_attention(q, c, n - 3, return_lse=True)
     for h in (0, H - 1):
-        _judge(q[:, h:h + 1], _head(c, h), [n - 3], out[:, h:h + 1], lse[:, h:h + 1], least=2.0 ** (-22 if kind == "near" else -25))
+        _check(q[:, h:h + 1], _head(c, h), [n - 3], out[:, h:h + 1], lse[:, h:h + 1], least=2.0 ** (-22 if kind == "near" else -25))
 
 
 @pytest.mark.parametrize("S", [1, 100])
@@ -167,7 +167,7 @@ def test_sparse_queries_beside_an_unanswered_value(device, scale):
     q = q.to(BF16)
     out, lse = cached_attention(q, c, n, sm_scale=scale, return_lse=True)
     for h in range(len(sizes)):
-        _judge(q[:, h:h + 1], _head(c, h), [n], out[:, h:h + 1], lse[:, h:h + 1], scale)
+        _check(q[:, h:h + 1], _head(c, h), [n], out[:, h:h + 1], lse[:, h:h + 1], scale)
 
 
 def test_an_infinite_query_over_a_long_walk(device):
